@@ -5,6 +5,7 @@
 #include <cstring>
 #include <c10/hip/HIPStream.h>
 #include <c10/hip/HIPCachingAllocator.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 
 #include "kernels/kernels.h"
 #include "kernels/conv_route.h"
@@ -1088,6 +1089,136 @@ void softmax_eval(Tensor logits, c10::optional<Tensor> labels, c10::optional<Ten
                       logits.size(0), logits.size(1), stream());
 }
 
+// ------------------------------------------------------------------------- label log-probabilities
+// rows of logits: [N, C] with unit column stride (a channel slice or padded rows are fine)
+void check_logit_rows(const Tensor& x, const char* who) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, who, ": logits [N, C] on the GPU");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), who, ": bf16 / fp32 logits");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (int64_t(1) << 31) - 64, who, ": 1 <= classes < 2^31 - 64");
+  TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, who, ": classes must be contiguous");
+  TORCH_CHECK(x.size(0) <= 1 || x.stride(0) >= x.size(1), who, ": rows must not overlap");
+}
+
+const int64_t* opt_row_labels(const c10::optional<Tensor>& t, const Tensor& x, const char* who) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->scalar_type() == torch::kInt64 && t->is_contiguous() && t->numel() == x.size(0) &&
+                  t->device() == x.device(), who, ": labels int64 [N] on the logits' device");
+  return t->data_ptr<int64_t>();
+}
+
+const float* opt_rows_f32(const c10::optional<Tensor>& t, const Tensor& x, int64_t n, const char* who) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(is_f32(*t) && t->is_contiguous() && t->numel() == n && t->device() == x.device(), who,
+              ": row gradients fp32, contiguous, on the logits' device");
+  return t->data_ptr<float>();
+}
+
+// -> (log_prob [N] or None, entropy [N], top_log_prob [N, k], top_index [N, k] or None, stat [N, 3]
+// or None)
+py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int64_t ignore,
+                          bool want_stat) {
+  check_logit_rows(x, "label_log_probs");
+  const int64_t N = x.size(0), C = x.size(1);
+  TORCH_CHECK(k >= 0 && k <= LOGPROB_MAX_K && k <= C, "label_log_probs: 0 <= top_k <= min(classes, ",
+              LOGPROB_MAX_K, ")");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  LogProbArgs a{};
+  a.labels = opt_row_labels(labels, x, "label_log_probs");
+  Tensor logp, top_lp, top_idx, stat, ps, pk;
+  Tensor ent = torch::empty({N}, f32);
+  if (a.labels) logp = torch::empty({N}, f32);
+  if (k) {
+    top_lp = torch::empty({N, k}, f32);
+    top_idx = torch::empty({N, k}, x.options().dtype(torch::kInt64));
+  }
+  if (want_stat) stat = torch::empty({N, 3}, f32);
+  if (N) {
+    const int parts = logprob_parts(N, C);
+    if (parts > 1) {
+      ps = torch::empty({N * parts * 3}, f32);
+      if (k) pk = torch::empty({N * parts * k}, x.options().dtype(torch::kInt64));
+    }
+    a.x = x.data_ptr();
+    a.ld = N > 1 ? x.stride(0) : C;
+    a.ignore = ignore;
+    a.N = N;
+    a.C = C;
+    a.k = (int)k;
+    a.logp = a.labels ? F32(logp) : nullptr;
+    a.ent = F32(ent);
+    if (k) {
+      a.top_lp = F32(top_lp);
+      a.top_idx = top_idx.data_ptr<int64_t>();
+    }
+    if (want_stat) a.stat = F32(stat);
+    if (parts > 1) {
+      a.part_stat = F32(ps);
+      if (k) a.part_key = reinterpret_cast<unsigned long long*>(pk.data_ptr<int64_t>());
+    }
+    logprob_launch(a, !is_f32(x), parts, stream());
+  }
+  auto opt = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
+  return py::make_tuple(opt(logp), ent, opt(top_lp), opt(top_idx), opt(stat));
+}
+
+Tensor label_log_probs_bwd(Tensor x, c10::optional<Tensor> labels, Tensor stat,
+                           c10::optional<Tensor> g_logp, c10::optional<Tensor> g_ent,
+                           c10::optional<Tensor> g_top, c10::optional<Tensor> top_idx,
+                           int64_t ignore) {
+  const char* who = "label_log_probs backward";
+  check_logit_rows(x, who);
+  const int64_t N = x.size(0), C = x.size(1);
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  LogProbGradArgs a{};
+  a.labels = opt_row_labels(labels, x, who);
+  a.stat = opt_rows_f32(stat, x, 3 * N, who);
+  a.g_logp = opt_rows_f32(g_logp, x, N, who);
+  a.g_ent = opt_rows_f32(g_ent, x, N, who);
+  if (g_top.has_value() && g_top->defined()) {
+    TORCH_CHECK(top_idx.has_value() && top_idx->scalar_type() == torch::kInt64 &&
+                    top_idx->is_contiguous() && top_idx->dim() == 2 && top_idx->size(0) == N &&
+                    top_idx->device() == x.device(), who, ": top_index int64 [N, k]");
+    a.k = (int)top_idx->size(1);
+    a.g_top = opt_rows_f32(g_top, x, N * a.k, who);
+    a.top_idx = top_idx->data_ptr<int64_t>();
+  }
+  Tensor dx = torch::empty({N, C}, x.options());
+  if (!N) return dx;
+  a.x = x.data_ptr();
+  a.ld = N > 1 ? x.stride(0) : C;
+  a.ignore = ignore;
+  a.N = N;
+  a.C = C;
+  a.dx = dx.data_ptr();
+  logprob_bwd_launch(a, !is_f32(x), stream());
+  return dx;
+}
+
+// ------------------------------------------------------------------------------------------ dropout
+Tensor dropout(Tensor x, Tensor key, int64_t cut, double scale) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous(), "dropout: contiguous HIP tensor");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), "dropout: bf16 / fp32");
+  TORCH_CHECK(key.scalar_type() == torch::kInt64 && key.numel() == 2 && key.is_contiguous() &&
+                  key.device() == x.device(), "dropout key: int64 [2] on the input's device");
+  TORCH_CHECK(cut >= 0 && cut <= 65536, "dropout: 0 <= cut <= 65536");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor y = torch::empty_like(x);
+  if (x.numel())
+    dropout_launch(x.data_ptr(), y.data_ptr(), x.numel(), !is_f32(x), key.data_ptr<int64_t>(),
+                   (uint32_t)cut, (float)scale, stream());
+  return y;
+}
+
+Tensor dropout_next_key(Tensor state) {
+  CHECK_T(state, torch::kInt64);
+  TORCH_CHECK(state.numel() == 2, "dropout key state: int64 [2]");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(state.device());
+  Tensor key = torch::empty_like(state);
+  dropout_next_key_launch(state.data_ptr<int64_t>(), key.data_ptr<int64_t>(), stream());
+  return key;
+}
+
 int label_kind(const Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return 0;
@@ -1693,6 +1824,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("loss_sum") = py::none(), py::arg("correct") = py::none(),
         py::arg("probs") = py::none());
   m.def("lovasz_hinge", &lovasz_hinge);
+  m.def("label_log_probs", &label_log_probs, py::arg("logits"), py::arg("labels"), py::arg("top_k"),
+        py::arg("ignore_index"), py::arg("want_stat"));
+  m.def("label_log_probs_bwd", &label_log_probs_bwd, py::arg("logits"), py::arg("labels"),
+        py::arg("stat"), py::arg("g_logp"), py::arg("g_ent"), py::arg("g_top"), py::arg("top_index"),
+        py::arg("ignore_index"));
+  m.def("dropout", &dropout, py::arg("x"), py::arg("key"), py::arg("cut"), py::arg("scale"));
+  m.def("dropout_next_key", &dropout_next_key, py::arg("state"));
   m.def("seg_metrics", &seg_metrics);
   m.def("sgd_momentum", &sgd_momentum, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("lowp"),
         py::arg("flags"), py::arg("lr"), py::arg("mu"), py::arg("wd"), py::arg("gs"),

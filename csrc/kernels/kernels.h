@@ -436,6 +436,46 @@ void upsample_bwd_launch(const float* dy, float* dx, const int* ih, const float*
                          const int* iw, const float* ww, int N, int H, int W, int C, int Ho,
                          int Wo, hipStream_t st, int ldd = 0);
 
+// log-probabilities of labels, entropy, top-k classes (logprob.hip); x [N][ld] bf16 / fp32
+constexpr int LOGPROB_SHORT = 2048;   // longest row that stays in one wave's registers
+constexpr int LOGPROB_MAX_PARTS = 64;
+constexpr int LOGPROB_MAX_K = 32;
+struct LogProbArgs {
+  const void* x;
+  long ld;
+  const int64_t* labels;  // null: no log-probabilities
+  long ignore;
+  long N, C;              // C < 2^31 − 64
+  int k;                  // ≤ min(C, LOGPROB_MAX_K)
+  float *logp, *ent;      // [N]
+  float* top_lp;          // [N][k]
+  int64_t* top_idx;
+  float* stat;            // [N][3] = (m, log s, H) for the backward pass, or null
+  float* part_stat;       // parts > 1: [N][parts][3]
+  unsigned long long* part_key;  // parts > 1 and k: [N][parts][k]
+};
+struct LogProbGradArgs {
+  const void* x;
+  long ld;
+  const int64_t* labels;
+  long ignore;
+  long N, C;
+  int k;
+  const float* stat;
+  const float *g_logp, *g_ent, *g_top;  // null: not differentiated
+  const int64_t* top_idx;
+  void* dx;               // [N][C], x's type
+};
+int logprob_parts(long N, long C);  // workgroups per row the forward will use
+void logprob_launch(const LogProbArgs& a, bool bf16, int parts, hipStream_t st);
+void logprob_bwd_launch(const LogProbGradArgs& a, bool bf16, hipStream_t st);
+
+// counter-based dropout (dropout.hip): y = keep ? x·scale : 0, 16 random bits per element
+void dropout_launch(const void* x, void* y, long n, bool bf16, const int64_t* key, uint32_t cut,
+                    float scale, hipStream_t st);
+// out = state, state[1] += 1 (one draw of a stream of keys)
+void dropout_next_key_launch(int64_t* state, int64_t* out, hipStream_t st);
+
 // fault injection: a 1-lane kernel that spins `ms` milliseconds (≤ 60 s) on stream st
 void debug_spin_launch(double ms, hipStream_t st);
 

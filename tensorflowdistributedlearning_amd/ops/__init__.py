@@ -3,6 +3,8 @@ from .conv import ConvGeom, conv2d, conv_fwd, conv_dgrad, conv_wgrad, same_paddi
 from .bn import batch_norm_act
 from .pool import max_pool2d, global_avg_pool
 from .loss import softmax_cross_entropy, lovasz_hinge
+from .logprob import label_log_probs, LabelLogProbs
+from .dropout import dropout, DropoutKeys
 from .dwconv import depthwise_conv2d, laplace
 from .upsample import upsample as upsample_bilinear_tf1
 from .elementwise import add_relu, relu, add, sigmoid_threshold
@@ -11,5 +13,6 @@ from . import optim
 
 __all__ = ["ConvGeom", "conv2d", "conv_fwd", "conv_dgrad", "conv_wgrad", "same_padding",
            "batch_norm_act", "max_pool2d", "global_avg_pool", "softmax_cross_entropy",
-           "lovasz_hinge", "depthwise_conv2d", "laplace", "upsample_bilinear_tf1", "add_relu", "relu", "add",
+           "lovasz_hinge", "label_log_probs", "LabelLogProbs", "dropout", "DropoutKeys",
+           "depthwise_conv2d", "laplace", "upsample_bilinear_tf1", "add_relu", "relu", "add",
            "sigmoid_threshold", "seg_scores", "StreamingMean", "IOU_THRESHOLDS", "optim"]
