@@ -64,10 +64,13 @@ def build(verbose=True, force=False):
               "-Wno-deprecated-declarations"]
     if os.environ.get("TDL_CONV_ABLATION") == "1":  # timing-only TDL_CONV_DBG flags (dev/tools/*_ablate.py)
         common.append("-DTDL_CONV_ABLATION=1")
+    # no packed fp32 instructions: some forms of them have given wrong results on gfx950 (the host
+    # pass warns that it does not know the feature)
+    device = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     for src in sorted(glob.glob(os.path.join(CSRC, "kernels", "*.hip"))):
         obj = os.path.join(OBJ, os.path.basename(src) + ".o")
         if force or _newer(src, obj, headers):
-            jobs.append([HIPCC, f"--offload-arch={ARCH}", *common, "-c", "-o", obj, src])
+            jobs.append([HIPCC, f"--offload-arch={ARCH}", *common, *device, "-c", "-o", obj, src])
     for src in sorted(glob.glob(os.path.join(CSRC, "runtime", "*.cpp"))):
         obj = os.path.join(OBJ, "rt_" + os.path.basename(src) + ".o")
         if force or _newer(src, obj, headers):
