@@ -9,6 +9,7 @@
 
 #include "kernels/kernels.h"
 #include "kernels/conv_route.h"
+#include "kernels/int8.h"
 #include "runtime/loader.h"
 #include "runtime/comm.h"
 
@@ -1219,6 +1220,70 @@ Tensor dropout_next_key(Tensor state) {
   return key;
 }
 
+// --------------------------------------------------------------------------------- 8-bit linear
+void check_int8_k(int64_t K, const char* who) {
+  TORCH_CHECK(K >= 1 && K <= INT8_MAX_K, who, ": 1 <= K <= ", INT8_MAX_K);
+}
+
+// x [M, K] bf16 / fp32, unit column stride -> (q: int8 blocks, csrc/kernels/int8.h; scale [M])
+std::tuple<Tensor, Tensor> int8_quantize(Tensor x) {
+  const char* who = "int8_quantize";
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, who, ": [M, K] on the GPU");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), who, ": bf16 / fp32");
+  const int64_t M = x.size(0), K = x.size(1);
+  check_int8_k(K, who);
+  TORCH_CHECK((K == 1 || x.stride(1) == 1) && (M <= 1 || x.stride(0) >= K), who,
+              ": contiguous, non-overlapping rows");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor q = torch::empty({int8_rows(M), int8_kp(K)}, x.options().dtype(torch::kInt8));
+  Tensor s = torch::empty({M}, x.options().dtype(torch::kFloat32));
+  if (M)
+    int8_quantize_launch(x.data_ptr(), M > 1 ? x.stride(0) : K, !is_f32(x), M, K,
+                         q.data_ptr<int8_t>(), F32(s), stream());
+  return {q, s};
+}
+
+// y [M, N] = act(scales · q wᵀ + bias [+ res]); q, w: int8 blocks of the same K
+void int8_gemm(Tensor q, Tensor qs, Tensor w, Tensor ws, int64_t K, c10::optional<Tensor> bias,
+               c10::optional<Tensor> res, bool relu, Tensor y) {
+  const char* who = "int8_gemm";
+  check_int8_k(K, who);
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), who, ": y [M, N] on the GPU");
+  TORCH_CHECK(y.scalar_type() == torch::kBFloat16 || is_f32(y), who, ": bf16 / fp32 y");
+  const int64_t M = y.size(0), N = y.size(1), Kp = int8_kp(K);
+  TORCH_CHECK(N < (int64_t(1) << 31) - 512, who, ": N too large");
+  auto operand = [&](const Tensor& t, int64_t rows, const char* what) {
+    CHECK_T(t, torch::kInt8);
+    TORCH_CHECK(t.device() == y.device() && t.numel() == int8_rows(rows) * Kp, who, ": ", what,
+                " blocks of ", rows, " x ", K);
+  };
+  auto vec = [&](const Tensor& t, int64_t n, const char* what) {
+    CHECK_T(t, torch::kFloat32);
+    TORCH_CHECK(t.device() == y.device() && t.numel() == n, who, ": ", what, " fp32 [", n, "]");
+    return F32(t);
+  };
+  operand(q, M, "activation");
+  operand(w, N, "weight");
+  Int8GemmArgs a{};
+  a.q = q.data_ptr<int8_t>();
+  a.w = w.data_ptr<int8_t>();
+  a.qs = vec(qs, M, "activation scales");
+  a.ws = vec(ws, N, "weight scales");
+  if (bias.has_value() && bias->defined()) a.bias = vec(*bias, N, "bias");
+  if (res.has_value() && res->defined()) {
+    TORCH_CHECK(res->device() == y.device() && res->is_contiguous() && res->sizes() == y.sizes() &&
+                    res->scalar_type() == y.scalar_type(), who, ": residual like y");
+    a.res = res->data_ptr();
+  }
+  a.y = y.data_ptr();
+  a.M = M;
+  a.N = (int)N;
+  a.Kp = (int)Kp;
+  a.relu = relu;
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(y.device());
+  if (M && N) int8_gemm_launch(a, !is_f32(y), stream());
+}
+
 int label_kind(const Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return 0;
@@ -1829,6 +1894,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("label_log_probs_bwd", &label_log_probs_bwd, py::arg("logits"), py::arg("labels"),
         py::arg("stat"), py::arg("g_logp"), py::arg("g_ent"), py::arg("g_top"), py::arg("top_index"),
         py::arg("ignore_index"));
+  m.def("int8_quantize", &int8_quantize, py::arg("x"));
+  m.def("int8_gemm", &int8_gemm, py::arg("q"), py::arg("qs"), py::arg("w"), py::arg("ws"), py::arg("K"),
+        py::arg("bias"), py::arg("res"), py::arg("relu"), py::arg("y"));
   m.def("dropout", &dropout, py::arg("x"), py::arg("key"), py::arg("cut"), py::arg("scale"));
   m.def("dropout_next_key", &dropout_next_key, py::arg("state"));
   m.def("seg_metrics", &seg_metrics);
