@@ -1243,45 +1243,88 @@ std::tuple<Tensor, Tensor> int8_quantize(Tensor x) {
   return {q, s};
 }
 
-// y [M, N] = act(scales · q wᵀ + bias [+ res]); q, w: int8 blocks of the same K
-void int8_gemm(Tensor q, Tensor qs, Tensor w, Tensor ws, int64_t K, c10::optional<Tensor> bias,
-               c10::optional<Tensor> res, bool relu, Tensor y) {
-  const char* who = "int8_gemm";
+// the arguments int8_gemm and int8_linear share: w blocks of [N, K], y [M, N]
+Int8GemmArgs int8_args(const Tensor& w, const Tensor& ws, int64_t K, const c10::optional<Tensor>& bias,
+                       const c10::optional<Tensor>& res, bool relu, const Tensor& y, const char* who) {
   check_int8_k(K, who);
-  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), who, ": y [M, N] on the GPU");
-  TORCH_CHECK(y.scalar_type() == torch::kBFloat16 || is_f32(y), who, ": bf16 / fp32 y");
-  const int64_t M = y.size(0), N = y.size(1), Kp = int8_kp(K);
+  const int64_t M = y.size(0), N = y.size(1);
   TORCH_CHECK(N < (int64_t(1) << 31) - 512, who, ": N too large");
-  auto operand = [&](const Tensor& t, int64_t rows, const char* what) {
-    CHECK_T(t, torch::kInt8);
-    TORCH_CHECK(t.device() == y.device() && t.numel() == int8_rows(rows) * Kp, who, ": ", what,
-                " blocks of ", rows, " x ", K);
-  };
-  auto vec = [&](const Tensor& t, int64_t n, const char* what) {
-    CHECK_T(t, torch::kFloat32);
-    TORCH_CHECK(t.device() == y.device() && t.numel() == n, who, ": ", what, " fp32 [", n, "]");
-    return F32(t);
-  };
-  operand(q, M, "activation");
-  operand(w, N, "weight");
+  CHECK_T(w, torch::kInt8);
+  CHECK_T(ws, torch::kFloat32);
+  TORCH_CHECK(w.device() == y.device() && w.numel() == int8_rows(N) * int8_kp(K), who,
+              ": weight blocks of ", N, " x ", K, " on x's device");
+  TORCH_CHECK(ws.device() == y.device() && ws.numel() == N, who, ": weight scales fp32 [", N, "]");
   Int8GemmArgs a{};
-  a.q = q.data_ptr<int8_t>();
   a.w = w.data_ptr<int8_t>();
-  a.qs = vec(qs, M, "activation scales");
-  a.ws = vec(ws, N, "weight scales");
-  if (bias.has_value() && bias->defined()) a.bias = vec(*bias, N, "bias");
+  a.ws = F32(ws);
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK(bias->device() == y.device() && is_f32(*bias) && bias->is_contiguous() &&
+                    bias->numel() == N, who, ": bias fp32 [", N, "] on x's device");
+    a.bias = F32(*bias);
+  }
   if (res.has_value() && res->defined()) {
-    TORCH_CHECK(res->device() == y.device() && res->is_contiguous() && res->sizes() == y.sizes() &&
+    TORCH_CHECK(res->device() == y.device() && res->is_contiguous() && res->numel() == M * N &&
                     res->scalar_type() == y.scalar_type(), who, ": residual like y");
     a.res = res->data_ptr();
   }
   a.y = y.data_ptr();
   a.M = M;
   a.N = (int)N;
-  a.Kp = (int)Kp;
+  a.Kp = (int)int8_kp(K);
   a.relu = relu;
+  return a;
+}
+
+// act(scales · q wᵀ + bias [+ res]) of already quantised rows, into y [M, N]
+void int8_gemm(Tensor q, Tensor qs, Tensor w, Tensor ws, int64_t K, c10::optional<Tensor> bias,
+               c10::optional<Tensor> res, bool relu, Tensor y) {
+  const char* who = "int8_gemm";
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), who, ": y [M, N] on the GPU");
+  TORCH_CHECK(y.scalar_type() == torch::kBFloat16 || is_f32(y), who, ": bf16 / fp32 y");
+  Int8GemmArgs a = int8_args(w, ws, K, bias, res, relu, y, who);
+  CHECK_T(q, torch::kInt8);
+  CHECK_T(qs, torch::kFloat32);
+  TORCH_CHECK(q.device() == y.device() && q.numel() == int8_rows(a.M) * a.Kp && qs.device() == y.device() &&
+                  qs.numel() == a.M, who, ": activation blocks and scales of ", a.M, " x ", K);
+  a.q = q.data_ptr<int8_t>();
+  a.qs = F32(qs);
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(y.device());
-  if (M && N) int8_gemm_launch(a, !is_f32(y), stream());
+  if (a.M && a.N) int8_gemm_launch(a, !is_f32(y), stream());
+}
+
+// x [..., K] bf16 / fp32 -> act(x wᵀ + bias [+ res]) [..., N] in x's type
+Tensor int8_linear(Tensor x, Tensor w, Tensor ws, int64_t N, c10::optional<Tensor> bias,
+                   c10::optional<Tensor> res, bool relu) {
+  const char* who = "int8_linear";
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1, who, ": [..., K] on the GPU");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), who, ": bf16 / fp32");
+  const int64_t K = x.size(-1);
+  check_int8_k(K, who);
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+  Tensor m = x.dim() == 2 ? x : x.reshape({-1, K});
+  const int64_t M = m.size(0);
+  if ((K > 1 && m.stride(1) != 1) || (M > 1 && m.stride(0) < K)) m = m.contiguous();
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  Tensor y = torch::empty(shape, x.options());
+  Tensor r;
+  if (res.has_value() && res->defined()) {
+    TORCH_CHECK(res->sizes() == y.sizes(), who, ": residual like the output");
+    r = res->contiguous();
+  }
+  const Tensor y2 = y.view({M, N});
+  const Int8GemmArgs a = int8_args(w, ws, K, bias, r.defined() ? c10::optional<Tensor>(r) : c10::nullopt,
+                                   relu, y2, who);
+  if (!M || !N) return y;
+  Tensor q, qs;
+  if (!int8_linear_fused(M, a.Kp)) {
+    q = torch::empty({int8_rows(M), a.Kp}, x.options().dtype(torch::kInt8));
+    qs = torch::empty({M}, x.options().dtype(torch::kFloat32));
+  }
+  int8_linear_launch(m.data_ptr(), M > 1 ? m.stride(0) : K, K, a,
+                     q.defined() ? q.data_ptr<int8_t>() : nullptr, qs.defined() ? F32(qs) : nullptr,
+                     !is_f32(x), stream());
+  return y;
 }
 
 int label_kind(const Tensor& t) {
@@ -1897,6 +1940,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_quantize", &int8_quantize, py::arg("x"));
   m.def("int8_gemm", &int8_gemm, py::arg("q"), py::arg("qs"), py::arg("w"), py::arg("ws"), py::arg("K"),
         py::arg("bias"), py::arg("res"), py::arg("relu"), py::arg("y"));
+  m.def("int8_linear", &int8_linear, py::arg("x"), py::arg("w"), py::arg("ws"), py::arg("N"),
+        py::arg("bias"), py::arg("res"), py::arg("relu"));
   m.def("dropout", &dropout, py::arg("x"), py::arg("key"), py::arg("cut"), py::arg("scale"));
   m.def("dropout_next_key", &dropout_next_key, py::arg("state"));
   m.def("seg_metrics", &seg_metrics);

@@ -29,6 +29,11 @@ struct Int8GemmArgs {
   int N, Kp;
   bool relu;
 };
+// quantise x's rows and multiply; q / qs: room for the blocks and scales, not touched when the
+// rows are few enough to be quantised where they are used (int8_linear_fused)
+bool int8_linear_fused(long M, long Kp);
+void int8_linear_launch(const void* x, long ld, long K, const Int8GemmArgs& a, int8_t* q, float* qs,
+                        bool bf16, hipStream_t st);
 void int8_gemm_launch(const Int8GemmArgs& a, bool bf16, hipStream_t st);
 
 }  // namespace tdl

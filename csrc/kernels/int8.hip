@@ -105,6 +105,14 @@ __device__ __forceinline__ int quant1<float>(float x, const RowScale& s) {
   return (int)q;
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t quant4(const float* f, const RowScale& r) {
+  uint32_t o = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o |= (uint32_t)(uint8_t)quant1<T>(f[j], r) << (8 * j);
+  return o;
+}
+
 // A workgroup of NW waves quantises 16 rows.  Lane l of a wave holds 16 elements of row l % 16 at
 // k = 64 b + 16 (l / 16): reads are 16 segments of 128 bytes, the write is one block of 1 KiB.
 // Wave w takes blocks w, w + NW, …; V of them stay in registers, longer rows are read twice.
@@ -162,12 +170,7 @@ __global__ void __launch_bounds__(64 * NW) quantize_kernel(const T* __restrict__
       raw.get(f);
       uint32_t o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[i] |= (uint32_t)(uint8_t)(bad ? 0 : quant1<T>(f[4 * i + j], rs)) << (8 * j);
-      }
+      for (int i = 0; i < 4; ++i) o[i] = bad ? 0u : quant4<T>(f + 4 * i, rs);
       *(uint4*)(q + (g * nb + b) * 1024 + lane * 16) = make_uint4(o[0], o[1], o[2], o[3]);
     };
     for (int b0 = w; b0 < nb; b0 += NW * V) {
@@ -189,128 +192,236 @@ __device__ __forceinline__ void wait_vmcnt() {
 }
 __device__ __forceinline__ void raw_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-// N fragments of 1 KiB each, consecutive in LDS; the wait is in the same block, so the registers
-// hold the data when the compiler may use them
-template <int N>
-__device__ __forceinline__ void lds_frags(i32x4 (&f)[N], uint32_t at);
-template <>
-__device__ __forceinline__ void lds_frags<4>(i32x4 (&f)[4], uint32_t at) {
-  asm volatile(
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
-      "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3])
-      : "v"(at)
-      : "memory");
+// One wave copies a block of 1 KiB into LDS at the wave-uniform address dst.  Written as assembly
+// so that the compiler does not wait for every copy in flight before each LDS read; the waits are
+// explicit (vmcnt, then a barrier).  No register is written.
+__device__ __forceinline__ void dma_block(rsrc_t r, uint32_t dst, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(dst), "v"(off), "s"(r)
+               : "memory", "m0");
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float* v, int left, bool vec);
-template <>
-__device__ __forceinline__ void store4<bf16_t>(bf16_t* p, const float* v, int left, bool vec) {
-  if (vec && left >= 4) {
-    *(uint2*)p = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) store1(p + i, v[i]);
-  }
+typedef __attribute__((address_space(3))) const i32x4 lds_i32x4;
+__device__ __forceinline__ i32x4 lds_frag(uint32_t at) { return *(lds_i32x4*)(uintptr_t)at; }
+
+// 8 outputs of a row as 16-byte pieces at any element alignment
+__device__ __forceinline__ void ld8u(const bf16_t* p, float* f) {
+  const q4_a2 v = *(const q4_a2*)p;
+  unpack8(make_uint4(v.x, v.y, v.z, v.w), f);
 }
-template <>
-__device__ __forceinline__ void store4<float>(float* p, const float* v, int left, bool vec) {
-  if (vec && left >= 4) {
-    *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) p[i] = v[i];
-  }
+__device__ __forceinline__ void ld8u(const float* p, float* f) {
+  const q4_a4 a = ((const q4_a4*)p)[0], b = ((const q4_a4*)p)[1];
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void st8u(bf16_t* p, const float* f) {
+  const uint4 v = pack8(f);
+  *(q4_a2*)p = q4_a2{v.x, v.y, v.z, v.w};
+}
+__device__ __forceinline__ void st8u(float* p, const float* f) {
+  ((q4_a4*)p)[0] = q4_a4{f[0], f[1], f[2], f[3]};
+  ((q4_a4*)p)[1] = q4_a4{f[4], f[5], f[6], f[7]};
 }
 
-// four outputs of one row from column n on
-template <typename T>
-__device__ __forceinline__ void finish4(const Int8GemmArgs& a, const i32x4& acc, long m, int n,
-                                        float qs, bool vec) {
-  if (m >= a.M || n >= a.N) return;
-  const int left = a.N - n;
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = i < left ? n + i : n;
-    v[i] = (float)acc[i] * (qs * a.ws[j]);
-    if (a.bias) v[i] += a.bias[j];
-  }
-  T* y = (T*)a.y + m * a.N + n;
-  if (a.res) {
-    const T* r = (const T*)a.res + m * a.N + n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) v[i] += load1(r + i);
-  }
-  if (a.relu) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
-  }
-  store4<T>(y, v, left, vec);
+// 16-row tiles to workgroups: XCD x takes a contiguous run (its L2 keeps what neighbours share),
+// ordered in groups of GM row tiles, down the rows first
+template <int GM>
+__device__ __forceinline__ void tile_of(int id, int tm, int tn, int* m, int* n) {
+  id = xcd_remap(id, tm * tn);
+  const int per = GM * tn, g = id / per, gm = min(GM, tm - g * GM), r = id - g * per;
+  *n = r / gm;
+  *m = g * GM + r - *n * gm;
 }
 
-// BM × BN outputs per workgroup, 64 × 64 per wave; ST stages of 64 k in LDS, filled by LDS-DMA
-// while the matrix unit works on the oldest.
-template <typename T, int BM, int BN, int ST>
-__global__ void __launch_bounds__(BM * BN / 64) gemm_kernel(Int8GemmArgs a) {
-  constexpr int NW = BM / 64 * (BN / 64), WN = BN / 64;
-  constexpr int BLK = (BM + BN) / 16, PER = BLK / NW;  // blocks of a stage, per wave
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// A wave's products on MF × MF tiles of the matrix unit (16×16×64 or 32×32×32; the weights are the
+// first operand, so a lane holds 4 consecutive columns of one row).  R rows × C columns of 16.
+template <int MF, int R, int C>
+struct Tile;
+template <int R, int C>
+struct Tile<16, R, C> {
+  i32x4 acc[R][C] = {};
+  // lane l: row l % 16, k = 16 (l / 16)
+  static __device__ __forceinline__ uint32_t lane_off(int l) { return l * 16; }
+  static __device__ __forceinline__ constexpr uint32_t frag_off(int i) { return i * 1024; }
+  __device__ __forceinline__ void products(const i32x4 (&a)[R], const i32x4 (&b)[C]) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j], a[i], acc[i][j], 0, 0, 0);
+  }
+  // row tile i to LDS: put(row in the tile, column, 4 values)
+  template <typename F>
+  __device__ __forceinline__ void each(int i, int l, F put) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) put(l & 15, j * 16 + (l >> 4) * 4, acc[i][j]);
+  }
+};
+template <int R, int C>
+struct Tile<32, R, C> {
+  i32x16 acc[R / 2][C / 2] = {};
+  // lane l: row l % 32, k = 16 (l / 32) of the 32 of a fragment; fragment i: rows 32 (i / 2), k half i % 2
+  static __device__ __forceinline__ uint32_t lane_off(int l) {
+    return ((l >> 4) & 1) * 1024 + (l >> 5) * 256 + (l & 15) * 16;
+  }
+  static __device__ __forceinline__ constexpr uint32_t frag_off(int i) { return (i >> 1) * 2048 + (i & 1) * 512; }
+  __device__ __forceinline__ void products(const i32x4 (&a)[R], const i32x4 (&b)[C]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i)
+#pragma unroll
+        for (int j = 0; j < C / 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[2 * j + h], a[2 * i + h], acc[i][j], 0, 0, 0);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(int i, int l, F put) {
+#pragma unroll
+    for (int j = 0; j < C / 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        put(l & 31, j * 32 + g * 8 + (l >> 5) * 4,
+            i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
+  }
+};
+
+// FM × FN blocks of 16 × 16 per wave, WM × WN waves, ST stages of 64 k in LDS.
+//
+// Step kt: the copies of stage kt + 1 have landed (vmcnt, barrier); stage kt + ST − 1 is copied into
+// the slot of stage kt − 1, whose fragments went into products before the barrier; the fragments of
+// kt + 1 are read while the products of kt run.  Copies past the end read zeros, which keeps the
+// count of copies in flight the same in every step.
+template <typename T, int MF, int FM, int FN, int WM, int WN, int ST>
+__global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
+  constexpr int NW = WM * WN, BM = FM * 16 * WM, BN = FN * 16 * WN;
+  constexpr int BLK = (BM + BN) / 16, PER = BLK / NW, STAGE = BLK * 1024;
   static_assert(BLK % NW == 0, "every wave moves the same number of blocks");
+  static_assert(ST >= 3, "");
   extern __shared__ char smem[];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nb = a.Kp / 64;
-  const int tn = (a.N + BN - 1) / BN;
-  const long m0 = (long)(blockIdx.x / tn) * BM;
-  const int n0 = (int)(blockIdx.x % tn) * BN;
+  const int tn = (a.N + BN - 1) / BN, tm = (int)((a.M + BM - 1) / BM);
+  int im, in;
+  tile_of<8>(blockIdx.x, tm, tn, &im, &in);
+  const long m0 = (long)im * BM;
+  const int n0 = in * BN;
   // rows past the end read as zeros: the descriptors end with the last whole block row
   const long mrows = min((long)BM, (a.M + 15) / 16 * 16 - m0);
   const int nrows = min(BN, (a.N + 15) / 16 * 16 - n0);
   const rsrc_t ra = make_rsrc(a.q + m0 * a.Kp, (uint32_t)(mrows * a.Kp));
   const rsrc_t rb = make_rsrc(a.w + (long)n0 * a.Kp, (uint32_t)((long)nrows * a.Kp));
-  auto issue = [&](int kt) {
-    char* stage = smem + (kt % ST) * (BLK * 1024);
+  const uint32_t base = (uint32_t)(uintptr_t)(lds_void_t*)smem;
+  uint32_t off[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int b = p * NW + w;  // 0 .. BM/16 − 1: activations, then weights
+    off[p] = (uint32_t)((b < BM / 16 ? b : b - BM / 16) * nb) * 1024u + lane * 16u;
+  }
+  auto issue = [&](int kt, int slot) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int b = p * NW + w;  // 0 .. BM/16 − 1: activations, then weights
-      const bool isa = b < BM / 16;
-      const int rb16 = isa ? b : b - BM / 16;
-      const uint32_t off = kt < nb ? (uint32_t)(rb16 * nb + kt) * 1024u + lane * 16u : 0xffffff00u;
-      lds_void_t* dst = (lds_void_t*)(stage + b * 1024);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(isa ? ra : rb, dst, 16, off, 0, 0, 0);
+      const int b = p * NW + w;
+      const uint32_t o = kt < nb ? off[p] + (uint32_t)kt * 1024u : convk::OOB;
+      const uint32_t dst = base + slot * STAGE + b * 1024;
+      if ((p + 1) * NW <= BM / 16) dma_block(ra, dst, o);
+      else if (p * NW >= BM / 16) dma_block(rb, dst, o);
+      else dma_block(b < BM / 16 ? ra : rb, dst, o);
     }
   };
-  i32x4 acc[4][4] = {};
+  using Acc = Tile<MF, FM, FN>;
+  Acc t;
   const int wm = w / WN, wn = w % WN;
-  for (int s = 0; s < ST - 1; ++s) issue(s);
-  const uint32_t base = (uint32_t)(uintptr_t)(lds_void_t*)smem;
-  for (int kt = 0; kt < nb; ++kt) {
-    wait_vmcnt<PER*(ST - 2)>();
+  const uint32_t fa0 = base + wm * FM * 1024 + Acc::lane_off(lane);
+  const uint32_t fb0 = base + (BM / 16) * 1024 + wn * FN * 1024 + Acc::lane_off(lane);
+  auto frags = [&](i32x4(&fa)[FM], i32x4(&fb)[FN], int slot) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[j] = lds_frag(fb0 + slot * STAGE + Acc::frag_off(j));
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[i] = lds_frag(fa0 + slot * STAGE + Acc::frag_off(i));
+  };
+  i32x4 xa[FM], xb[FN], ya[FM], yb[FN];
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) issue(s, s);
+  wait_vmcnt<PER*(ST - 2)>();
+  raw_barrier();
+  frags(xa, xb, 0);
+  int slot = 0;  // of stage kt
+  auto next = [](int s) { return s + 1 == ST ? 0 : s + 1; };
+  auto step = [&](int kt, const i32x4(&fa)[FM], const i32x4(&fb)[FN], i32x4(&ga)[FM], i32x4(&gb)[FN]) {
+    // no product of the step before moves below the barrier: its fragments' slot is refilled here
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<PER*(ST - 3)>();
     raw_barrier();
-    issue(kt + ST - 1);  // past the end: zeros into a slot nobody reads, and the count stays even
-    const uint32_t st = base + (kt % ST) * (BLK * 1024) + lane * 16;
-    i32x4 fa[4], fb[4];
-    lds_frags<4>(fa, st + wm * 4096);
-    lds_frags<4>(fb, st + (BM / 16) * 1024 + wn * 4096);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+    issue(kt + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+    slot = next(slot);
+    frags(ga, gb, slot);
+    t.products(fa, fb);
+  };
+  // Kp is a multiple of 128: an even number of stages
+  for (int kt = 0; kt < nb; kt += 2) {
+    step(kt, xa, xb, ya, yb);
+    step(kt + 1, ya, yb, xa, xb);
   }
-  wait_vmcnt<0>();  // no copy into LDS outlives the workgroup
-  const bool vec = a.N % 4 == 0 && (uintptr_t)a.y % 16 == 0;
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vmcnt<0>();  // no copy into LDS outlives the loop
+  raw_barrier();
+
+  // Epilogue, MF rows at a time through the wave's own part of LDS: the matrix unit leaves 4 columns
+  // of one row in a lane, memory wants whole rows.  Lane l then finishes 8 columns of a row.
+  constexpr int CPR = FN * 2, RPI = 64 / CPR, PITCH = FN * 64 + 16;  // lanes per row, rows per pass
+  const uint32_t ep = base + w * MF * PITCH;
+  const int col = n0 + wn * FN * 16 + lane % CPR * 8;
+  const int left = a.N - col;
+  float ws[8], bias[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long m = m0 + wm * 64 + i * 16 + (lane & 15);
-    const float qs = m < a.M ? a.qs[m] : 0.f;
+  for (int e = 0; e < 8; ++e) {
+    const bool in = e < left;
+    ws[e] = in ? a.ws[col + e] : 0.f;
+    bias[e] = in && a.bias ? a.bias[col + e] : 0.f;
+  }
+  const long row0 = m0 + wm * FM * 16 + lane / CPR;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      finish4<T>(a, acc[i][j], m, n0 + wn * 64 + j * 16 + (lane >> 4) * 4, qs, vec);
+  for (int i = 0; i < FM * 16 / MF; ++i) {
+    t.each(i, lane, [&](int r, int c, const i32x4& v) {
+      *(__attribute__((address_space(3))) i32x4*)(uintptr_t)(ep + r * PITCH + c * 4) = v;
+    });
+#pragma unroll
+    for (int r = 0; r < MF; r += RPI) {
+      const uint32_t at = ep + (r + lane / CPR) * PITCH + lane % CPR * 32;
+      const i32x4 lo = lds_frag(at), hi = lds_frag(at + 16);
+      const long m = row0 + i * MF + r;
+      if (m >= a.M || left <= 0) continue;
+      const float qs = a.qs[m];
+      float v[8], add[8];
+      T* y = (T*)a.y + m * a.N + col;
+      const T* res = (const T*)a.res + m * a.N + col;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add[e] = 0.f;
+      if (a.res) {
+        if (left >= 8) {
+          ld8u(res, add);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) add[e] = load1(res + e);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = (float)(e < 4 ? lo[e] : hi[e - 4]) * (qs * ws[e]) + bias[e] + add[e];
+        v[e] = a.relu && p < 0.f ? 0.f : p;  // NaN stays NaN
+      }
+      if (left >= 8) {
+        st8u(y, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) store1(y + e, v[e]);
+      }
+    }
   }
 }
 
@@ -324,14 +435,192 @@ void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipS
   else quantize_kernel<T, 16, 4, true><<<grid, 1024, 0, st>>>(x, ld, M, K, nb, q, scale);
 }
 
+// ------------------------------------------------------------------------------- few rows
+// Up to 16 MB rows: the weights are read once, straight into registers in the order the matrix unit
+// takes them, so the kernel is a stream over them.  A workgroup owns 16 output channels; its NW
+// waves take the blocks of 64 k in turn, U loads of 1 KiB in flight each, and add their sums in LDS.
+//
+// FUSED (x in its own type instead of quantised blocks): every workgroup quantises the few rows
+// itself, under the latency of its first weight loads.  With one to four rows that is 16 elements
+// per thread or so; a launch of its own costs more (FUSED_ROWS, FUSED_ITEMS below).
+constexpr int FUSED_ROWS = 4, FUSED_ITEMS = 4;
+
+template <typename T, int MB, int NW, bool FUSED>
+__global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T* __restrict__ x,
+                                                         long ld, long K) {
+  constexpr int U = 8;
+  static_assert(!FUSED || MB == 1, "");
+  extern __shared__ char smem[];  // FUSED: quantised rows, [Kp / 16][M][16 bytes]
+  __shared__ i32x4 part[NW][MB][64];
+  __shared__ uint32_t tops[FUSED_ROWS];
+  __shared__ float scales[FUSED_ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int nb = a.Kp / 64, M = (int)a.M;
+  const int n0 = blockIdx.x * 16;
+  const i32x4* wp = (const i32x4*)(a.w + (long)blockIdx.x * 16 * a.Kp) + lane;
+  i32x4 wr[U];
+  auto fetch = [&](int kb0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kb0 + u * NW < nb) wr[u] = wp[(long)(kb0 + u * NW) * 64];
+  };
+  fetch(w);
+  if (FUSED) {
+    const int kc = a.Kp / 16, items = M * kc;
+    if (tid < FUSED_ROWS) tops[tid] = 0;
+    __syncthreads();
+    // items past the end hold zeros of the last row: every lane stays in the wave's reductions
+    Raw16<T> d[FUSED_ITEMS];
+    int row[FUSED_ITEMS], ck[FUSED_ITEMS];
+#pragma unroll
+    for (int i = 0; i < FUSED_ITEMS; ++i) {
+      const int item = tid + i * 64 * NW;
+      row[i] = item < items ? item / kc : M - 1;
+      ck[i] = item < items ? item - row[i] * kc : kc;
+      d[i].load(x + row[i] * ld + ck[i] * 16, K - ck[i] * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < FUSED_ITEMS; ++i) {
+      float f[16], top = 0.f;
+      d[i].get(f);
+      bool fin = true;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        top = fmaxf(top, fabsf(f[e]));
+        fin = fin && fabsf(f[e]) < INFINITY;
+      }
+      if (!fin) top = INFINITY;
+      // one atomic per wave where the wave is within a row (floats ≥ 0 order like their bits)
+      const int row0 = __builtin_amdgcn_readfirstlane(row[i]);
+      if (__all(row[i] == row0)) {
+        top = wave_max(top);
+        if (lane == 0) atomicMax(&tops[row0], __float_as_uint(top));
+      } else {
+        atomicMax(&tops[row[i]], __float_as_uint(top));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FUSED_ITEMS; ++i) {
+      if (ck[i] >= kc) continue;
+      const float top = fmaxf(__uint_as_float(tops[row[i]]), TINY);
+      const bool bad = top == INFINITY;
+      if (ck[i] == 0) scales[row[i]] = bad ? NAN : top / 127.f;
+      const RowScale rs = row_scale(top);
+      float f[16];
+      d[i].get(f);
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = bad ? 0u : quant4<T>(f + 4 * j, rs);
+      ((uint4*)smem)[ck[i] * M + row[i]] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __syncthreads();
+  }
+  i32x4 acc[MB] = {};
+  const int r = lane & 15, c = lane >> 4;
+  const i32x4* qp = (const i32x4*)a.q + lane;
+  for (int kb0 = w; kb0 < nb; kb0 += NW * U) {
+    if (kb0 != w) fetch(kb0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kb = kb0 + u * NW;
+      if (kb >= nb) break;
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        // rows past the last one repeat it: their sums are not stored
+        const i32x4 q = FUSED ? ((const i32x4*)smem)[(kb * 4 + c) * M + min(r, M - 1)]
+                              : m * 16 < M ? qp[((long)m * nb + kb) * 64] : i32x4{};
+        acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wr[u], q, acc[m], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m) part[w][m][lane] = acc[m];
+  __syncthreads();
+  // lane l of a sum holds channels 4 (l / 16) … + 3 of row l % 16
+  for (int o = tid; o < MB * 256; o += 64 * NW) {
+    const int row = o >> 4, ch = o & 15, n = n0 + ch;
+    if (row >= M || n >= a.N) continue;
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) sum += part[i][row >> 4][(ch >> 2) * 16 + (row & 15)][ch & 3];
+    const float qs = FUSED ? scales[row] : a.qs[row];
+    const long at = (long)row * a.N + n;
+    float v = (float)sum * (qs * a.ws[n]) + (a.bias ? a.bias[n] : 0.f) +
+              (a.res ? load1((const T*)a.res + at) : 0.f);
+    if (a.relu && v < 0.f) v = 0.f;
+    store1((T*)a.y + at, v);
+  }
+}
+
+template <typename T, int MF, int FM, int FN, int WM, int WN, int ST>
+void run_gemm(const Int8GemmArgs& a, hipStream_t st) {
+  constexpr int BM = FM * 16 * WM, BN = FN * 16 * WN, ring = ST * (BM + BN) * 64,
+                epi = WM * WN * MF * (FN * 64 + 16), lds = ring > epi ? ring : epi;
+  static const bool set = hipFuncSetAttribute((const void*)gemm_kernel<T, MF, FM, FN, WM, WN, ST>,
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+  (void)set;
+  const long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  gemm_kernel<T, MF, FM, FN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, lds, st>>>(a);
+}
+
+template <typename T, int MB, int NW, bool FUSED>
+void run_stream(const Int8GemmArgs& a, const T* x, long ld, long K, hipStream_t st) {
+  const int lds = FUSED ? (int)(a.M * a.Kp) : 0;
+  if (FUSED) {
+    static const bool set = hipFuncSetAttribute((const void*)stream_kernel<T, MB, NW, FUSED>,
+                                                hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                FUSED_ITEMS * 1024 * 16) == hipSuccess;
+    (void)set;
+  }
+  stream_kernel<T, MB, NW, FUSED><<<(unsigned)((a.N + 15) / 16), 64 * NW, lds, st>>>(a, x, ld, K);
+}
+
+constexpr long STREAM_ROWS = 64;
+
 template <typename T>
 void gemm(const Int8GemmArgs& a, hipStream_t st) {
-  const long tiles = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-  constexpr int lds = 4 * 16 * 1024;
-  gemm_kernel<T, 128, 128, 4><<<(unsigned)tiles, 256, lds, st>>>(a);
+  if (a.M <= STREAM_ROWS) {
+    const bool wide = a.Kp > 64 * 64;
+    if (a.M <= 16) wide ? run_stream<T, 1, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 1, 8, false>(a, nullptr, 0, 0, st);
+    else if (a.M <= 32) wide ? run_stream<T, 2, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 2, 8, false>(a, nullptr, 0, 0, st);
+    else wide ? run_stream<T, 4, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 4, 8, false>(a, nullptr, 0, 0, st);
+    return;
+  }
+  auto tiles = [&](long bm, long bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
+  // Large tiles read LDS least (8192³: 515 us, 128 × 128 tiles 582) but fill the chip late and leave
+  // one workgroup per CU, which short sums do not hide (50176 × 256 → 1024: 73 us against 55).
+  // 64 × 64 where 128 × 128 gives less than a tile to every other CU (512 × 2048 → 1000: 7.8 us
+  // against 11.0; 2049 × 1999 → 1003: 13.4 against 12.6).  The 32×32×32 form of the matrix unit
+  // needs fewer LDS reads in flight and wins on the small tiles (128 × 128: 14.3 against 19.5 us).
+  if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 16, 8, 4, 2, 4, 4>(a, st);
+  else if (tiles(128, 128) >= 128) run_gemm<T, 32, 4, 2, 2, 4, 4>(a, st);
+  else run_gemm<T, 32, 2, 2, 2, 2, 6>(a, st);
+}
+
+template <typename T>
+void linear(const T* x, long ld, long K, Int8GemmArgs a, int8_t* q, float* qs, hipStream_t st) {
+  const int items = (int)(a.M * (a.Kp / 16));
+  if (a.M <= FUSED_ROWS && items <= FUSED_ITEMS * 1024) {
+    if (items <= FUSED_ITEMS * 512 && a.Kp <= 64 * 64) run_stream<T, 1, 8, true>(a, x, ld, K, st);
+    else run_stream<T, 1, 16, true>(a, x, ld, K, st);
+    return;
+  }
+  quantize(x, ld, a.M, K, q, qs, st);
+  a.q = q;
+  a.qs = qs;
+  gemm<T>(a, st);
 }
 
 }  // namespace
+
+bool int8_linear_fused(long M, long Kp) { return M <= FUSED_ROWS && M * (Kp / 16) <= FUSED_ITEMS * 1024; }
+
+void int8_linear_launch(const void* x, long ld, long K, const Int8GemmArgs& a, int8_t* q, float* qs,
+                        bool bf16, hipStream_t st) {
+  if (bf16) linear((const bf16_t*)x, ld, K, a, q, qs, st);
+  else linear((const float*)x, ld, K, a, q, qs, st);
+}
 
 void int8_quantize_launch(const void* x, long ld, bool bf16, long M, long K, int8_t* q,
                           float* scale, hipStream_t st) {

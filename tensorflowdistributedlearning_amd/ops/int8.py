@@ -99,25 +99,24 @@ class Int8Rows:
         return (q.float() * self.scale[:, None]).view(self.shape)
 
 
-def _rows2d(x, who):
+def _check_rows(x, who):
     if x.dim() < 1:
         raise ValueError(f"{who}: x [..., K], got a scalar")
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype != torch.bfloat16 and x.dtype != torch.float32:
         raise TypeError(f"{who}: bf16 / fp32 activations, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who}: inference only (torch.no_grad(), or a tensor without gradient)")
     _check_k(x.shape[-1])
-    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
-        m = m.contiguous()
-    return m
 
 
 def quantize_rows(x):
     """Rows of ``x`` [..., K] (bf16 / fp32) in 8 bits with one scale each: :class:`Int8Rows`, for
     :func:`int8_linear` calls that share them."""
-    m = _rows2d(x, "quantize_rows")
+    _check_rows(x, "quantize_rows")
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if on_gpu(m):
+        if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+            m = m.contiguous()
         blocks, scale = ext().int8_quantize(m)
     else:
         q, scale = ref_quantize_rows(m)
@@ -134,23 +133,29 @@ def int8_linear(x, weight, bias=None, residual=None, relu=False):
     if not isinstance(weight, Int8Weight):
         raise TypeError(f"int8_linear: weight is an Int8Weight, got {type(weight).__name__}")
     rows = x if isinstance(x, Int8Rows) else None
+    if rows is None:
+        _check_rows(x, "int8_linear")
     if x.shape[-1] != weight.k:
         raise ValueError(f"int8_linear: x has K = {x.shape[-1]}, the weight {weight.k}")
-    device = (rows.scale if rows is not None else x).device
+    device = (x if rows is None else rows.scale).device
     if device != weight.device:
         raise ValueError(f"int8_linear: x on {device}, weight on {weight.device}")
-    out_shape = tuple(x.shape[:-1]) + (weight.n,)
     if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (weight.n,) or bias.device != device:
+        if bias.dtype != torch.float32 or bias.shape != (weight.n,) or bias.device != device:
             raise ValueError(f"int8_linear: bias fp32 [{weight.n}] on {device}, got {bias.dtype} "
                              f"{tuple(bias.shape)} on {bias.device}")
         bias = bias.detach().contiguous()
     if residual is not None:
-        if tuple(residual.shape) != out_shape or residual.dtype != x.dtype or residual.device != device:
+        out_shape = (*x.shape[:-1], weight.n)
+        if residual.shape != out_shape or residual.dtype != x.dtype or residual.device != device:
             raise ValueError(f"int8_linear: residual {x.dtype} {out_shape} on {device}, got "
                              f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
         if residual.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("int8_linear: inference only")
+    if rows is None and device.type == "cuda":
+        return ext().int8_linear(x, weight.blocks, weight.scale, weight.n, bias, residual, relu)
+    out_shape = (*x.shape[:-1], weight.n)
+    if residual is not None:
         residual = residual.reshape(-1, weight.n).contiguous()
     if rows is None:
         rows = quantize_rows(x)
@@ -158,7 +163,7 @@ def int8_linear(x, weight, bias=None, residual=None, relu=False):
     if device.type == "cuda":
         y = torch.empty(m, weight.n, dtype=x.dtype, device=device)
         ext().int8_gemm(rows.blocks, rows.scale, weight.blocks, weight.scale, weight.k, bias,
-                        residual, bool(relu), y)
+                        residual, relu, y)
         return y.view(out_shape)
     q = from_blocks(rows.blocks, m, weight.k).double()
     acc = (q @ from_blocks(weight.blocks, weight.n, weight.k).double().t()).float()
