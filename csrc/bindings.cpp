@@ -6,6 +6,8 @@
 #include <c10/hip/HIPStream.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "kernels/kernels.h"
 #include "kernels/conv_route.h"
@@ -1114,10 +1116,12 @@ const float* opt_rows_f32(const c10::optional<Tensor>& t, const Tensor& x, int64
   return t->data_ptr<float>();
 }
 
-// -> (log_prob [N] or None, entropy [N], top_log_prob [N, k], top_index [N, k] or None, stat [N, 3]
-// or None)
-py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int64_t ignore,
-                          bool want_stat) {
+struct LogProbOut {
+  Tensor logp, ent, top_lp, top_idx, stat;  // undefined where not asked for
+};
+
+LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& labels, int64_t k,
+                               int64_t ignore, bool want_stat) {
   check_logit_rows(x, "label_log_probs");
   const int64_t N = x.size(0), C = x.size(1);
   TORCH_CHECK(k >= 0 && k <= LOGPROB_MAX_K && k <= C, "label_log_probs: 0 <= top_k <= min(classes, ",
@@ -1126,41 +1130,38 @@ py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int
   const auto f32 = x.options().dtype(torch::kFloat32);
   LogProbArgs a{};
   a.labels = opt_row_labels(labels, x, "label_log_probs");
-  Tensor logp, top_lp, top_idx, stat, ps, pk;
-  Tensor ent = torch::empty({N}, f32);
-  if (a.labels) logp = torch::empty({N}, f32);
+  LogProbOut o;
+  Tensor ps, pk;
+  o.ent = torch::empty({N}, f32);
+  if (a.labels) o.logp = torch::empty({N}, f32);
   if (k) {
-    top_lp = torch::empty({N, k}, f32);
-    top_idx = torch::empty({N, k}, x.options().dtype(torch::kInt64));
+    o.top_lp = torch::empty({N, k}, f32);
+    o.top_idx = torch::empty({N, k}, x.options().dtype(torch::kInt64));
   }
-  if (want_stat) stat = torch::empty({N, 3}, f32);
-  if (N) {
-    const int parts = logprob_parts(N, C);
-    if (parts > 1) {
-      ps = torch::empty({N * parts * 3}, f32);
-      if (k) pk = torch::empty({N * parts * k}, x.options().dtype(torch::kInt64));
-    }
-    a.x = x.data_ptr();
-    a.ld = N > 1 ? x.stride(0) : C;
-    a.ignore = ignore;
-    a.N = N;
-    a.C = C;
-    a.k = (int)k;
-    a.logp = a.labels ? F32(logp) : nullptr;
-    a.ent = F32(ent);
-    if (k) {
-      a.top_lp = F32(top_lp);
-      a.top_idx = top_idx.data_ptr<int64_t>();
-    }
-    if (want_stat) a.stat = F32(stat);
-    if (parts > 1) {
-      a.part_stat = F32(ps);
-      if (k) a.part_key = reinterpret_cast<unsigned long long*>(pk.data_ptr<int64_t>());
-    }
-    logprob_launch(a, !is_f32(x), parts, stream());
+  if (want_stat) o.stat = torch::empty({N, 3}, f32);
+  if (!N) return o;
+  const int parts = logprob_parts(N, C);
+  if (parts > 1) {
+    ps = torch::empty({N * parts * 3}, f32);
+    if (k) pk = torch::empty({N * parts * k}, x.options().dtype(torch::kInt64));
+    a.part_stat = F32(ps);
+    if (k) a.part_key = reinterpret_cast<unsigned long long*>(pk.data_ptr<int64_t>());
   }
-  auto opt = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
-  return py::make_tuple(opt(logp), ent, opt(top_lp), opt(top_idx), opt(stat));
+  a.x = x.data_ptr();
+  a.ld = N > 1 ? x.stride(0) : C;
+  a.ignore = ignore;
+  a.N = N;
+  a.C = C;
+  a.k = (int)k;
+  a.logp = a.labels ? F32(o.logp) : nullptr;
+  a.ent = F32(o.ent);
+  if (k) {
+    a.top_lp = F32(o.top_lp);
+    a.top_idx = o.top_idx.data_ptr<int64_t>();
+  }
+  if (want_stat) a.stat = F32(o.stat);
+  logprob_launch(a, !is_f32(x), parts, stream());
+  return o;
 }
 
 Tensor label_log_probs_bwd(Tensor x, c10::optional<Tensor> labels, Tensor stat,
@@ -1196,19 +1197,113 @@ Tensor label_log_probs_bwd(Tensor x, c10::optional<Tensor> labels, Tensor stat,
   return dx;
 }
 
+// The autograd node is native: one training step through the operator costs two kernel launches and
+// little else (as a Python Function 60 us of host time, many times the kernels at small sizes).
+struct LabelLogProbsFn : torch::autograd::Function<LabelLogProbsFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
+                                                const c10::optional<Tensor>& labels, int64_t k,
+                                                int64_t ignore) {
+    LogProbOut o = label_log_probs_fwd(x, labels, k, ignore, true);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["ignore"] = ignore;
+    ctx->save_for_backward({x, labels.value_or(Tensor()), o.stat, o.top_idx});
+    if (k) ctx->mark_non_differentiable({o.top_idx});
+    torch::autograd::variable_list out{o.ent};
+    if (o.logp.defined()) out.push_back(o.logp);
+    if (k) {
+      out.push_back(o.top_lp);
+      out.push_back(o.top_idx);
+    }
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &labels = saved[1], &stat = saved[2], &idx = saved[3];
+    auto rows = [](const Tensor& t) {
+      return t.defined() ? c10::optional<Tensor>(t.to(torch::kFloat32).contiguous()) : c10::nullopt;
+    };
+    const bool lab = labels.defined();
+    const size_t top = lab ? 2 : 1;
+    const auto g_top = idx.defined() ? rows(g[top]) : c10::nullopt;
+    torch::autograd::variable_list dx;
+    {
+      at::AutoGradMode off(false);
+      dx.push_back(label_log_probs_bwd(
+          x, lab ? c10::optional<Tensor>(labels) : c10::nullopt, stat, lab ? rows(g[1]) : c10::nullopt,
+          rows(g[0]), g_top, g_top ? c10::optional<Tensor>(idx) : c10::nullopt,
+          ctx->saved_data["ignore"].toInt()));
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: an error where it is differentiated again
+      dx[0].requires_grad_(true);
+      dx = (*std::make_shared<torch::autograd::DelayedError>(
+          "label_log_probs is differentiable once", 1))(std::move(dx));
+    }
+    return {dx[0], Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// -> (log_prob [N] or None, entropy [N], top_log_prob [N, k], top_index [N, k] or None)
+py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int64_t ignore) {
+  Tensor logp, ent, top_lp, top_idx;
+  if (x.requires_grad() && at::GradMode::is_enabled()) {
+    const auto o = LabelLogProbsFn::apply(x, labels, k, ignore);
+    size_t i = 0;
+    ent = o[i++];
+    if (labels.has_value()) logp = o[i++];
+    if (k) {
+      top_lp = o[i++];
+      top_idx = o[i++];
+    }
+  } else {
+    LogProbOut o = label_log_probs_fwd(x, labels, k, ignore, false);
+    logp = o.logp, ent = o.ent, top_lp = o.top_lp, top_idx = o.top_idx;
+  }
+  auto opt = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
+  return py::make_tuple(opt(logp), ent, opt(top_lp), opt(top_idx));
+}
+
 // ------------------------------------------------------------------------------------------ dropout
-Tensor dropout(Tensor x, Tensor key, int64_t cut, double scale) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous(), "dropout: contiguous HIP tensor");
-  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), "dropout: bf16 / fp32");
-  TORCH_CHECK(key.scalar_type() == torch::kInt64 && key.numel() == 2 && key.is_contiguous() &&
-                  key.device() == x.device(), "dropout key: int64 [2] on the input's device");
-  TORCH_CHECK(cut >= 0 && cut <= 65536, "dropout: 0 <= cut <= 65536");
+Tensor dropout_run(const Tensor& x0, const Tensor& key, int64_t cut) {
+  const Tensor x = x0.contiguous();
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
   Tensor y = torch::empty_like(x);
+  const float scale = cut < 65536 ? 65536.f / (float)(65536 - cut) : 0.f;
   if (x.numel())
     dropout_launch(x.data_ptr(), y.data_ptr(), x.numel(), !is_f32(x), key.data_ptr<int64_t>(),
-                   (uint32_t)cut, (float)scale, stream());
+                   (uint32_t)cut, scale, stream());
   return y;
+}
+
+// linear in x: the gradient is the same operator on dy (differentiable again by the same rule)
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& key,
+                        int64_t cut) {
+    ctx->save_for_backward({key});
+    ctx->saved_data["cut"] = cut;
+    return dropout_run(x, key, cut);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const Tensor key = ctx->get_saved_variables()[0];
+    const int64_t cut = ctx->saved_data["cut"].toInt();
+    Tensor dx = g[0];
+    if (dx.defined())
+      dx = dx.requires_grad() && at::GradMode::is_enabled() ? DropoutFn::apply(dx, key, cut)
+                                                            : dropout_run(dx, key, cut);
+    return {dx, Tensor(), Tensor()};
+  }
+};
+
+Tensor dropout(Tensor x, Tensor key, int64_t cut) {
+  TORCH_CHECK(x.is_cuda(), "dropout: HIP tensor");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), "dropout: bf16 / fp32");
+  TORCH_CHECK(key.scalar_type() == torch::kInt64 && key.numel() == 2 && key.is_contiguous() &&
+                  key.device() == x.device(), "dropout key: contiguous int64 [2] on the input's device");
+  TORCH_CHECK(cut >= 0 && cut <= 65536, "dropout: 0 <= cut <= 65536");
+  return x.requires_grad() && at::GradMode::is_enabled() ? DropoutFn::apply(x, key, cut)
+                                                         : dropout_run(x, key, cut);
 }
 
 Tensor dropout_next_key(Tensor state) {
@@ -1933,16 +2028,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("probs") = py::none());
   m.def("lovasz_hinge", &lovasz_hinge);
   m.def("label_log_probs", &label_log_probs, py::arg("logits"), py::arg("labels"), py::arg("top_k"),
-        py::arg("ignore_index"), py::arg("want_stat"));
-  m.def("label_log_probs_bwd", &label_log_probs_bwd, py::arg("logits"), py::arg("labels"),
-        py::arg("stat"), py::arg("g_logp"), py::arg("g_ent"), py::arg("g_top"), py::arg("top_index"),
         py::arg("ignore_index"));
   m.def("int8_quantize", &int8_quantize, py::arg("x"));
   m.def("int8_gemm", &int8_gemm, py::arg("q"), py::arg("qs"), py::arg("w"), py::arg("ws"), py::arg("K"),
         py::arg("bias"), py::arg("res"), py::arg("relu"), py::arg("y"));
   m.def("int8_linear", &int8_linear, py::arg("x"), py::arg("w"), py::arg("ws"), py::arg("N"),
         py::arg("bias"), py::arg("res"), py::arg("relu"));
-  m.def("dropout", &dropout, py::arg("x"), py::arg("key"), py::arg("cut"), py::arg("scale"));
+  m.def("dropout", &dropout, py::arg("x"), py::arg("key"), py::arg("cut"));
   m.def("dropout_next_key", &dropout_next_key, py::arg("state"));
   m.def("seg_metrics", &seg_metrics);
   m.def("sgd_momentum", &sgd_momentum, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("lowp"),

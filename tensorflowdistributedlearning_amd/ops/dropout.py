@@ -44,21 +44,21 @@ def ref_dropout_keep(numel, p, key):
     return bits >= _cut(p)
 
 
-def _run(x, cut, key):
-    scale = 65536.0 / (65536 - cut) if cut < 65536 else 0.0
+def _ref_dropout(x, cut, key):
     x = x.contiguous()
-    if on_gpu(x):
-        return ext().dropout(x, key, cut, scale)
     keep = ref_dropout_keep(x.numel(), cut / 65536, key).view(x.shape)
+    scale = 65536.0 / (65536 - cut) if cut < 65536 else 0.0
     return torch.where(keep, x.float() * scale, torch.zeros((), device=x.device)).to(x.dtype)
 
 
 class _DropoutFn(torch.autograd.Function):
+    """The CPU path's autograd node (the GPU's is native, csrc/bindings.cpp DropoutFn)."""
+
     @staticmethod
     def forward(ctx, x, cut, key):
         ctx.cut = cut
         ctx.save_for_backward(key)
-        return _run(x, cut, key)
+        return _ref_dropout(x, cut, key)
 
     @staticmethod
     def backward(ctx, dy):
@@ -82,9 +82,7 @@ def dropout(x, p, key):
     if cut == 0:
         return x
     key = key.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
-        return _DropoutFn.apply(x, cut, key)
-    return _run(x, cut, key)
+    return ext().dropout(x, key, cut) if on_gpu(x) else _DropoutFn.apply(x, cut, key)
 
 
 class DropoutKeys:

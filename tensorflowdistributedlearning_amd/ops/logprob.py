@@ -66,29 +66,6 @@ def ref_label_log_probs(logits, labels=None, top_k=0, ignore_index=-100, dtype=t
     return LabelLogProbs(logp, ent, tlp, ti)
 
 
-class _LabelLogProbsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, labels, top_k, ignore_index):
-        logp, ent, tlp, ti, stat = ext().label_log_probs(x, labels, top_k, ignore_index, True)
-        ctx.set_materialize_grads(False)
-        ctx.ignore_index = ignore_index
-        ctx.save_for_backward(x, labels, stat, ti)
-        if ti is not None:
-            ctx.mark_non_differentiable(ti)
-        return logp, ent, tlp, ti
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logp, g_ent, g_top, _):
-        x, labels, stat, ti = ctx.saved_tensors
-
-        def rows(g):
-            return None if g is None else g.float().contiguous()
-        dx = ext().label_log_probs_bwd(x, labels, stat, rows(g_logp), rows(g_ent), rows(g_top),
-                                       ti if g_top is not None else None, ctx.ignore_index)
-        return dx, None, None, None
-
-
 def label_log_probs(logits, labels=None, top_k=0, ignore_index=-100):
     """Log-probability of each row's label, the entropy of its distribution and its ``top_k`` most
     probable classes.
@@ -126,10 +103,7 @@ def label_log_probs(logits, labels=None, top_k=0, ignore_index=-100):
     if (C > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < C):
         x = x.contiguous()
     lab = None if labels is None else labels.reshape(-1).contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        out = _LabelLogProbsFn.apply(x, lab, int(top_k), int(ignore_index))
-    else:
-        out = ext().label_log_probs(x, lab, int(top_k), int(ignore_index), False)[:4]
+    out = ext().label_log_probs(x, lab, int(top_k), int(ignore_index))  # with its autograd node
     if flat:
         return LabelLogProbs(*out)
     return LabelLogProbs(*(None if t is None else t.reshape(lead + t.shape[1:]) for t in out))
