@@ -152,6 +152,8 @@ def main():
                     help="GPU compute precision: bf16 (fused bf16 kernels, fp32 accumulation / "
                          "master weights) or fp32 (fp32 operands on the fp32 MFMA end to end — the "
                          "reference's own precision, for the like-for-like deeplab_ref comparison)")
+    ap.add_argument("--int8", action="store_true",
+                    help="with --mode infer: linear layers in 8 bits (models.enable_int8)")
     ap.add_argument("--mode", choices=("train", "infer"), default="train",
                     help="train (the headline: full training step) or infer (serving: eval-mode "
                          "forward under no_grad with every BatchNorm folded into its conv, "
@@ -262,6 +264,8 @@ def main():
                   + ("bf16" if gpu_bf16 else "fp32")
                   + (" (BN unfolded)" if args.no_fold else " (BN folded into the convs)"))
         cfg.update(optimizer=None, loss=None, mode="infer", bn_folded=not args.no_fold)
+        if args.int8:
+            cfg["int8_layers"] = models.enable_int8(model)
         base = None
 
         @torch.no_grad()

@@ -1412,7 +1412,7 @@ Tensor int8_linear(Tensor x, Tensor w, Tensor ws, int64_t N, c10::optional<Tenso
                                    relu, y2, who);
   if (!M || !N) return y;
   Tensor q, qs;
-  if (!int8_linear_fused(M, a.Kp)) {
+  if (!int8_linear_fused(M, a.Kp, !is_f32(x))) {
     q = torch::empty({int8_rows(M), a.Kp}, x.options().dtype(torch::kInt8));
     qs = torch::empty({M}, x.options().dtype(torch::kFloat32));
   }

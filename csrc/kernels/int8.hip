@@ -9,6 +9,8 @@
 #include "conv_common.h"
 #include "int8.h"
 
+#include <type_traits>
+
 namespace tdl {
 namespace {
 
@@ -24,6 +26,9 @@ constexpr float TINY = 0x1p-40f;
 
 struct __attribute__((packed, aligned(2))) q4_a2 { uint32_t x, y, z, w; };
 struct __attribute__((packed, aligned(4))) q4_a4 { float x, y, z, w; };
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+constexpr uint32_t INF_BITS = 0x7f800000u;
 
 // 16 elements of a row as stored (any element alignment), the row's end filled with zeros
 template <typename T>
@@ -50,6 +55,15 @@ struct Raw16<bf16_t> {
     unpack8(v[0], f);
     unpack8(v[1], f + 8);
   }
+  // max |x| as the bits of a float: in integer order NaN is above infinity above every number
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    return (uint32_t)max(m[0], m[1]) << 16;
+  }
 };
 template <>
 struct Raw16<float> {
@@ -70,6 +84,12 @@ struct Raw16<float> {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f[i] = v[i];
   }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
 };
 
 // q = rint(127 x / top), exactly rounded (ties to even) in both types.  c127 = 127·2^-64 and top is
@@ -78,7 +98,8 @@ struct Raw16<float> {
 // itself away from the middle of two steps unless it is the middle.  Corrected once by its
 // remainder it has an error of 2^-23 of itself and returns a representable quotient, which a middle
 // is, exactly: every case is decided.
-// fp32: the remainder 127 x − q top has 31 bits, exact in 64; it tells whether q is the nearest.
+// fp32: a quotient that is not within 2^-13 of a middle has the right nearest integer (its error is
+// below 127·2^-22); else the remainder 127 x − q top, 31 bits, exact in 64, tells.
 struct RowScale {
   float top, rtop, c127;
 };
@@ -86,31 +107,35 @@ __device__ __forceinline__ RowScale row_scale(float top) {
   const float s = top >= 0x1p64f ? 0x1p-64f : 1.f;
   return RowScale{top * s, 1.f / (top * s), 127.f * s};
 }
+// the result's low byte is q: adding 1.5·2^23 rounds to the nearest integer, ties to even, and
+// leaves it in the low bits
 template <typename T>
-__device__ __forceinline__ int quant1(float x, const RowScale& r);
+__device__ __forceinline__ uint32_t quant1(float x, const RowScale& r);
 template <>
-__device__ __forceinline__ int quant1<bf16_t>(float x, const RowScale& r) {
+__device__ __forceinline__ uint32_t quant1<bf16_t>(float x, const RowScale& r) {
   const float n = r.c127 * x;
   float q = n * r.rtop;
   q = fmaf(fmaf(-q, r.top, n), r.rtop, q);
-  return (int)rintf(q);
+  return __float_as_uint(q + 12582912.f);
 }
 template <>
-__device__ __forceinline__ int quant1<float>(float x, const RowScale& s) {
-  float q = rintf((s.c127 * x) * s.rtop);
-  const double top = s.top, half = 0.5 * top, r = fma(-(double)q, top, (double)s.c127 * (double)x);
-  const bool odd = (int)q & 1;
-  if (r > half || (r == half && odd)) q += 1.f;
-  if (r < -half || (r == -half && odd)) q -= 1.f;
-  return (int)q;
+__device__ __forceinline__ uint32_t quant1<float>(float x, const RowScale& s) {
+  const float t = (s.c127 * x) * s.rtop;
+  float q = rintf(t);
+  if (!(fabsf(t - q) < 0.5f - 0x1p-13f)) {
+    const double top = s.top, half = 0.5 * top, r = fma(-(double)q, top, (double)s.c127 * (double)x);
+    const bool odd = (int)q & 1;
+    if (r > half || (r == half && odd)) q += 1.f;
+    if (r < -half || (r == -half && odd)) q -= 1.f;
+  }
+  return __float_as_uint(q + 12582912.f);
 }
-
 template <typename T>
 __device__ __forceinline__ uint32_t quant4(const float* f, const RowScale& r) {
-  uint32_t o = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o |= (uint32_t)(uint8_t)quant1<T>(f[j], r) << (8 * j);
-  return o;
+  const uint32_t a = quant1<T>(f[0], r), b = quant1<T>(f[1], r), c = quant1<T>(f[2], r), d = quant1<T>(f[3], r);
+  // bytes: 0–3 of the second operand, 4–7 of the first
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                               0x05040100u);
 }
 
 // A workgroup of NW waves quantises 16 rows.  Lane l of a wave holds 16 elements of row l % 16 at
@@ -120,7 +145,7 @@ template <typename T, int NW, int V, bool LONG>
 __global__ void __launch_bounds__(64 * NW) quantize_kernel(const T* __restrict__ x, long ld, long M,
                                                            long K, int nb, int8_t* __restrict__ q,
                                                            float* __restrict__ scale) {
-  __shared__ float sh[NW][16];
+  __shared__ uint32_t sh[NW][16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
   const long groups = (M + 15) / 16;
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
@@ -128,20 +153,10 @@ __global__ void __launch_bounds__(64 * NW) quantize_kernel(const T* __restrict__
     const bool live = row < M;
     const T* xr = x + (live ? row : 0) * ld;
     Raw16<T> d[V];
-    float top = 0.f;
-    bool fin = true;
+    uint32_t bits = 0;
     auto fetch = [&](Raw16<T>& raw, int b) {
       const long k = (long)b * 64 + c * 16;
       raw.load(xr + k, live ? K - k : 0);
-    };
-    auto scan = [&](const Raw16<T>& raw) {
-      float f[16];
-      raw.get(f);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        top = fmaxf(top, fabsf(f[i]));
-        fin = fin && fabsf(f[i]) < INFINITY;
-      }
     };
     for (int b0 = w; b0 < nb; b0 += NW * V) {
 #pragma unroll
@@ -149,20 +164,19 @@ __global__ void __launch_bounds__(64 * NW) quantize_kernel(const T* __restrict__
         if (b0 + v * NW < nb) fetch(d[v], b0 + v * NW);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (b0 + v * NW < nb) scan(d[v]);
+        if (b0 + v * NW < nb) bits = max(bits, d[v].top());
       if (!LONG) break;
     }
-    // a NaN or an infinity makes the row's scale NaN: it cannot be held in 8 bits
-    if (!fin) top = INFINITY;
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    bits = max(bits, __shfl_xor(bits, 16, 64));
+    bits = max(bits, __shfl_xor(bits, 32, 64));
     __syncthreads();
-    if (lane < 16) sh[w][lane] = top;
+    if (lane < 16) sh[w][lane] = bits;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NW; ++i) top = fmaxf(top, sh[i][r]);
-    top = fmaxf(top, TINY);
-    const bool bad = top == INFINITY;
+    for (int i = 0; i < NW; ++i) bits = max(bits, sh[i][r]);
+    // a NaN or an infinity makes the row's scale NaN: it cannot be held in 8 bits
+    const bool bad = bits >= INF_BITS;
+    const float top = fmaxf(__uint_as_float(bits), TINY);
     if (threadIdx.x < 16 && live) scale[row] = bad ? NAN : top / 127.f;
     const RowScale rs = row_scale(top);
     auto emit = [&](const Raw16<T>& raw, int b) {
@@ -205,11 +219,45 @@ __device__ __forceinline__ void dma_block(rsrc_t r, uint32_t dst, uint32_t off) 
 typedef __attribute__((address_space(3))) const i32x4 lds_i32x4;
 __device__ __forceinline__ i32x4 lds_frag(uint32_t at) { return *(lds_i32x4*)(uintptr_t)at; }
 
-// 8 outputs of a row as 16-byte pieces at any element alignment
-__device__ __forceinline__ void ld8u(const bf16_t* p, float* f) {
-  const q4_a2 v = *(const q4_a2*)p;
-  unpack8(make_uint4(v.x, v.y, v.z, v.w), f);
-}
+// 8 elements of a row at any element alignment, as stored; the first `left` of them are the row's
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<bf16_t> {
+  uint4 v;
+  __device__ __forceinline__ void load(const bf16_t* p, int left) {
+    if (left >= 8) {
+      const q4_a2 a = *(const q4_a2*)p;
+      v = make_uint4(a.x, a.y, a.z, a.w);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (2 * i < left ? (uint32_t)p[2 * i] : 0u) |
+               (2 * i + 1 < left ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ void get(float* f) const { unpack8(v, f); }
+};
+template <>
+struct Raw8<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p, int left) {
+    if (left >= 8) {
+      const q4_a4 a = ((const q4_a4*)p)[0], b = ((const q4_a4*)p)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = v[i];
+  }
+};
 __device__ __forceinline__ void ld8u(const float* p, float* f) {
   const q4_a4 a = ((const q4_a4*)p)[0], b = ((const q4_a4*)p)[1];
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
@@ -294,7 +342,7 @@ struct Tile<32, R, C> {
 // the slot of stage kt − 1, whose fragments went into products before the barrier; the fragments of
 // kt + 1 are read while the products of kt run.  Copies past the end read zeros, which keeps the
 // count of copies in flight the same in every step.
-template <typename T, int MF, int FM, int FN, int WM, int WN, int ST>
+template <typename T, int GM, int MF, int FM, int FN, int WM, int WN, int ST>
 __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   constexpr int NW = WM * WN, BM = FM * 16 * WM, BN = FN * 16 * WN;
   constexpr int BLK = (BM + BN) / 16, PER = BLK / NW, STAGE = BLK * 1024;
@@ -305,7 +353,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   const int nb = a.Kp / 64;
   const int tn = (a.N + BN - 1) / BN, tm = (int)((a.M + BM - 1) / BM);
   int im, in;
-  tile_of<8>(blockIdx.x, tm, tn, &im, &in);
+  tile_of<GM>(blockIdx.x, tm, tn, &im, &in);
   const long m0 = (long)im * BM;
   const int n0 = in * BN;
   // rows past the end read as zeros: the descriptors end with the last whole block row
@@ -345,6 +393,42 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   i32x4 xa[FM], xb[FN], ya[FM], yb[FN];
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) issue(s, s);
+  // Epilogue layout (below): lane l finishes 8 columns of row l / CPR of each pass.  Its scales and
+  // biases are loaded behind the first copies (one after the other behind the products they cost
+  // more than a short sum), and on small tiles the residual, for which large ones have no registers.
+  constexpr int CPR = FN * 2, RPI = 64 / CPR, PASSES = FM * 16 / RPI;
+  constexpr bool PRE = PASSES * 8 * sizeof(T) <= 128;
+  const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
+  const int col = n0 + wn * FN * 16 + lane % CPR * 8;
+  const int left = a.N - col;
+  const long row0 = m0 + wm * FM * 16 + lane / CPR;
+  const T* res0 = (const T*)a.res + row0 * a.N + col;
+  float ws[8], bias[8] = {}, qs[PASSES];
+  Raw8<T> res[PRE ? PASSES : 1];
+  if (inside) {
+    ld8u(a.ws + col, ws);
+    if (a.bias) ld8u(a.bias + col, bias);
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) qs[p] = a.qs[row0 + p * RPI];
+    if (PRE && a.res) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) res[p].load(res0 + (long)p * RPI * a.N, 8);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = min(col + e, a.N - 1);
+      ws[e] = a.ws[c];
+      if (a.bias) bias[e] = a.bias[c];
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) qs[p] = a.qs[min(row0 + p * RPI, a.M - 1)];
+    if (PRE && a.res) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p)
+        res[p].load(res0 + (long)p * RPI * a.N, row0 + p * RPI < a.M ? left : 0);
+    }
+  }
   wait_vmcnt<PER*(ST - 2)>();
   raw_barrier();
   frags(xa, xb, 0);
@@ -370,59 +454,50 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   raw_barrier();
 
   // Epilogue, MF rows at a time through the wave's own part of LDS: the matrix unit leaves 4 columns
-  // of one row in a lane, memory wants whole rows.  Lane l then finishes 8 columns of a row.
-  constexpr int CPR = FN * 2, RPI = 64 / CPR, PITCH = FN * 64 + 16;  // lanes per row, rows per pass
+  // of one row in a lane, memory wants whole rows.
+  constexpr int PITCH = FN * 64 + 16;
   const uint32_t ep = base + w * MF * PITCH;
-  const int col = n0 + wn * FN * 16 + lane % CPR * 8;
-  const int left = a.N - col;
-  float ws[8], bias[8];
+  T* y0 = (T*)a.y + row0 * a.N + col;
+  auto finish = [&](auto whole) {  // whole: the tile lies inside y
+    constexpr bool W = decltype(whole)::value;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool in = e < left;
-    ws[e] = in ? a.ws[col + e] : 0.f;
-    bias[e] = in && a.bias ? a.bias[col + e] : 0.f;
-  }
-  const long row0 = m0 + wm * FM * 16 + lane / CPR;
+    for (int i = 0; i < FM * 16 / MF; ++i) {
+      t.each(i, lane, [&](int r, int c, const i32x4& v) {
+        *(__attribute__((address_space(3))) i32x4*)(uintptr_t)(ep + r * PITCH + c * 4) = v;
+      });
 #pragma unroll
-  for (int i = 0; i < FM * 16 / MF; ++i) {
-    t.each(i, lane, [&](int r, int c, const i32x4& v) {
-      *(__attribute__((address_space(3))) i32x4*)(uintptr_t)(ep + r * PITCH + c * 4) = v;
-    });
+      for (int r = 0; r < MF; r += RPI) {
+        const uint32_t at = ep + (r + lane / CPR) * PITCH + lane % CPR * 32;
+        const i32x4 lo = lds_frag(at), hi = lds_frag(at + 16);
+        const int pass = (i * MF + r) / RPI;
+        if (!W && (row0 + i * MF + r >= a.M || left <= 0)) continue;
+        const long d = (long)(i * MF + r) * a.N;
+        float v[8];
 #pragma unroll
-    for (int r = 0; r < MF; r += RPI) {
-      const uint32_t at = ep + (r + lane / CPR) * PITCH + lane % CPR * 32;
-      const i32x4 lo = lds_frag(at), hi = lds_frag(at + 16);
-      const long m = row0 + i * MF + r;
-      if (m >= a.M || left <= 0) continue;
-      const float qs = a.qs[m];
-      float v[8], add[8];
-      T* y = (T*)a.y + m * a.N + col;
-      const T* res = (const T*)a.res + m * a.N + col;
+        for (int e = 0; e < 8; ++e) v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]) * (qs[pass] * ws[e]) + bias[e];
+        if (a.res) {
+          float add[8];
+          if (!PRE) res[0].load(res0 + d, W ? 8 : left);
+          res[PRE ? pass : 0].get(add);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) add[e] = 0.f;
-      if (a.res) {
-        if (left >= 8) {
-          ld8u(res, add);
+          for (int e = 0; e < 8; ++e) v[e] += add[e];
+        }
+        if (a.relu) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays NaN
+        }
+        if (W || left >= 8) {
+          st8u(y0 + d, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (e < left) add[e] = load1(res + e);
+            if (e < left) store1(y0 + d + e, v[e]);
         }
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = (float)(e < 4 ? lo[e] : hi[e - 4]) * (qs * ws[e]) + bias[e] + add[e];
-        v[e] = a.relu && p < 0.f ? 0.f : p;  // NaN stays NaN
-      }
-      if (left >= 8) {
-        st8u(y, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < left) store1(y + e, v[e]);
-      }
     }
-  }
+  };
+  if (inside) finish(std::true_type());
+  else finish(std::false_type());
 }
 
 template <typename T>
@@ -430,9 +505,18 @@ void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipS
   const int nb = (int)(int8_kp(K) / 64);
   const long groups = (M + 15) / 16;
   const unsigned grid = (unsigned)(groups < (1 << 20) ? groups : (1 << 20));
-  if (nb <= 4 * 8) quantize_kernel<T, 4, 8, false><<<grid, 256, 0, st>>>(x, ld, M, K, nb, q, scale);
-  else if (nb <= 8 * 8) quantize_kernel<T, 8, 8, false><<<grid, 512, 0, st>>>(x, ld, M, K, nb, q, scale);
-  else quantize_kernel<T, 16, 4, true><<<grid, 1024, 0, st>>>(x, ld, M, K, nb, q, scale);
+  // waves enough that each holds few blocks: 16 rows alone are little work for a workgroup
+#define QUANT(NW, V, LONG)                                                                      \
+  return quantize_kernel<T, NW, V, LONG><<<grid, 64 * NW, 0, st>>>(x, ld, M, K, nb, q, scale)
+  if (nb <= 4) QUANT(4, 1, false);
+  if (nb <= 8) QUANT(8, 1, false);
+  if (nb <= 16) QUANT(16, 1, false);
+  if (nb <= 32) QUANT(16, 2, false);
+  if (nb <= 64) QUANT(16, 4, false);
+  if constexpr (sizeof(T) == 2)  // (fp32: more registers than there are)
+    if (nb <= 128) QUANT(16, 8, false);
+  QUANT(16, 4, true);
+#undef QUANT
 }
 
 // ------------------------------------------------------------------------------- few rows
@@ -474,6 +558,7 @@ __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T
     int row[FUSED_ITEMS], ck[FUSED_ITEMS];
 #pragma unroll
     for (int i = 0; i < FUSED_ITEMS; ++i) {
+      if (i * 64 * NW >= items) break;
       const int item = tid + i * 64 * NW;
       row[i] = item < items ? item / kc : M - 1;
       ck[i] = item < items ? item - row[i] * kc : kc;
@@ -481,30 +566,25 @@ __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T
     }
 #pragma unroll
     for (int i = 0; i < FUSED_ITEMS; ++i) {
-      float f[16], top = 0.f;
-      d[i].get(f);
-      bool fin = true;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        top = fmaxf(top, fabsf(f[e]));
-        fin = fin && fabsf(f[e]) < INFINITY;
-      }
-      if (!fin) top = INFINITY;
-      // one atomic per wave where the wave is within a row (floats ≥ 0 order like their bits)
+      if (i * 64 * NW >= items) break;
+      uint32_t bits = d[i].top();
+      // one atomic per wave where the wave is within a row 
       const int row0 = __builtin_amdgcn_readfirstlane(row[i]);
       if (__all(row[i] == row0)) {
-        top = wave_max(top);
-        if (lane == 0) atomicMax(&tops[row0], __float_as_uint(top));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) bits = max(bits, __shfl_xor(bits, o, 64));
+        if (lane == 0) atomicMax(&tops[row0], bits);
       } else {
-        atomicMax(&tops[row[i]], __float_as_uint(top));
+        atomicMax(&tops[row[i]], bits);
       }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < FUSED_ITEMS; ++i) {
+      if (i * 64 * NW >= items) break;
       if (ck[i] >= kc) continue;
+      const bool bad = tops[row[i]] >= INF_BITS;
       const float top = fmaxf(__uint_as_float(tops[row[i]]), TINY);
-      const bool bad = top == INFINITY;
       if (ck[i] == 0) scales[row[i]] = bad ? NAN : top / 127.f;
       const RowScale rs = row_scale(top);
       float f[16];
@@ -553,15 +633,15 @@ __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T
   }
 }
 
-template <typename T, int MF, int FM, int FN, int WM, int WN, int ST>
+template <typename T, int GM, int MF, int FM, int FN, int WM, int WN, int ST>
 void run_gemm(const Int8GemmArgs& a, hipStream_t st) {
   constexpr int BM = FM * 16 * WM, BN = FN * 16 * WN, ring = ST * (BM + BN) * 64,
                 epi = WM * WN * MF * (FN * 64 + 16), lds = ring > epi ? ring : epi;
-  static const bool set = hipFuncSetAttribute((const void*)gemm_kernel<T, MF, FM, FN, WM, WN, ST>,
+  static const bool set = hipFuncSetAttribute((const void*)gemm_kernel<T, GM, MF, FM, FN, WM, WN, ST>,
                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
   (void)set;
   const long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  gemm_kernel<T, MF, FM, FN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, lds, st>>>(a);
+  gemm_kernel<T, GM, MF, FM, FN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, lds, st>>>(a);
 }
 
 template <typename T, int MB, int NW, bool FUSED>
@@ -593,18 +673,26 @@ void gemm(const Int8GemmArgs& a, hipStream_t st) {
   // 64 × 64 where 128 × 128 gives less than a tile to every other CU (512 × 2048 → 1000: 7.8 us
   // against 11.0; 2049 × 1999 → 1003: 13.4 against 12.6).  The 32×32×32 form of the matrix unit
   // needs fewer LDS reads in flight and wins on the small tiles (128 × 128: 14.3 against 19.5 us).
-  if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 16, 8, 4, 2, 4, 4>(a, st);
-  else if (tiles(128, 128) >= 128) run_gemm<T, 32, 4, 2, 2, 4, 4>(a, st);
-  else run_gemm<T, 32, 2, 2, 2, 2, 6>(a, st);
+  if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 8, 16, 8, 4, 2, 4, 4>(a, st);
+  else if (tiles(128, 128) >= 128) run_gemm<T, 8, 32, 4, 2, 2, 4, 4>(a, st);
+  else run_gemm<T, 8, 32, 2, 2, 2, 2, 6>(a, st);
 }
+
+}  // namespace
+
+// (fp32 holds half as many items in its registers)
+bool int8_linear_fused(long M, long Kp, bool bf16) {
+  return M <= FUSED_ROWS && M * (Kp / 16) <= FUSED_ITEMS * (bf16 ? 1024 : 512);
+}
+
+namespace {
 
 template <typename T>
 void linear(const T* x, long ld, long K, Int8GemmArgs a, int8_t* q, float* qs, hipStream_t st) {
-  const int items = (int)(a.M * (a.Kp / 16));
-  if (a.M <= FUSED_ROWS && items <= FUSED_ITEMS * 1024) {
-    if (items <= FUSED_ITEMS * 512 && a.Kp <= 64 * 64) run_stream<T, 1, 8, true>(a, x, ld, K, st);
-    else run_stream<T, 1, 16, true>(a, x, ld, K, st);
-    return;
+  if (int8_linear_fused(a.M, a.Kp, sizeof(T) == 2)) {
+    if (a.M * (a.Kp / 16) <= FUSED_ITEMS * 512 && (a.Kp <= 64 * 64 || sizeof(T) == 4))
+      return run_stream<T, 1, 8, true>(a, x, ld, K, st);
+    if constexpr (sizeof(T) == 2) return run_stream<T, 1, 16, true>(a, x, ld, K, st);
   }
   quantize(x, ld, a.M, K, q, qs, st);
   a.q = q;
@@ -613,8 +701,6 @@ void linear(const T* x, long ld, long K, Int8GemmArgs a, int8_t* q, float* qs, h
 }
 
 }  // namespace
-
-bool int8_linear_fused(long M, long Kp) { return M <= FUSED_ROWS && M * (Kp / 16) <= FUSED_ITEMS * 1024; }
 
 void int8_linear_launch(const void* x, long ld, long K, const Int8GemmArgs& a, int8_t* q, float* qs,
                         bool bf16, hipStream_t st) {

@@ -152,6 +152,11 @@ def main(argv=None):
         p.add_argument("--num-samples", dest="num_samples", type=int, default=1024)
         p.add_argument("--max-folds", dest="max_folds", type=int)
         p.add_argument("--fp8", action="store_true", default=None)
+        p.add_argument("--dropout", type=float, help="classifiers: of the pooled features")
+        p.add_argument("--entropy-weight", dest="entropy_weight", type=float,
+                       help="classifiers: entropy term of the training loss")
+        p.add_argument("--int8", action="store_true", default=None,
+                       help="classifiers: 8-bit linear layers in predictions")
         p.add_argument("--hip-graph", dest="hip_graph", choices=("auto", "off"))
         p.add_argument("--save-checkpoints-steps", dest="save_checkpoints_steps", type=int)
         p.add_argument("--save-summary-steps", dest="save_summary_steps", type=int)

@@ -68,6 +68,9 @@ class ModelConfig:
     lr_warmup_steps: int = 0
     synthetic: bool = False           # classifiers: learnable synthetic dataset (sample ids)
     fp8: bool = False                 # classifiers: fp8 forward GEMMs
+    dropout: float = 0.0              # classifiers: of the pooled features, in training
+    entropy_weight: float = 0.0       # classifiers: entropy term of the training loss
+    int8: bool = False                # classifiers: 8-bit linear layers in predictions
     hip_graph: str = "auto"           # capture each fold's step as a HIP graph (GPU)
     eval_batches: Optional[int] = None
     max_folds: Optional[int] = None   # train only the first k folds

@@ -57,7 +57,9 @@ from .engine import schedules
 from .models.deeplab import DeepLabResNet
 from . import models as _models
 from .models.params import FlatParams
-from .ops.loss import lovasz_hinge, softmax_cross_entropy, softmax_eval
+from .ops.logprob import label_log_probs, MAX_TOP_K
+from .ops.loss import (confidence_penalty_cross_entropy, lovasz_hinge, softmax_cross_entropy,
+                       softmax_eval)
 from .ops.metrics import seg_scores, StreamingMean
 from .ops.optim import exponential_decay
 from .preprocessing.preprocessing import _prepare_directory, create_symlinks, TRAIN, EVAL
@@ -95,7 +97,8 @@ def network_from_config(cfg):
     arch = cfg.get("arch", "deeplab_ref")
     if arch in CLASSIFIER_ARCHS:
         return _models.build(arch, num_classes=cfg["num_classes"],
-                             in_channels=cfg.get("image_channels", 3))
+                             in_channels=cfg.get("image_channels", 3),
+                             dropout=cfg.get("dropout", 0.0))
     return DeepLabResNet(model_name=cfg["model_name"], in_channels=2,
                          output_stride=cfg["output_stride"], base_depth=cfg["base_depth"],
                          input_shape=tuple(cfg["input_shape"]), n_blocks=tuple(cfg["n_blocks"]),
@@ -168,6 +171,15 @@ class Model:
         self.lr_warmup_steps = kwargs.get("lr_warmup_steps", 0)
         self.synthetic = kwargs.get("synthetic", False)
         self.fp8 = kwargs.get("fp8", False)
+        # classifiers: dropout of the pooled features, weight of the entropy term of the loss
+        # (ops/loss.confidence_penalty_cross_entropy), 8-bit linear layers in predictions
+        self.dropout = float(kwargs.get("dropout", 0.0))
+        self.entropy_weight = float(kwargs.get("entropy_weight", 0.0))
+        self.int8 = bool(kwargs.get("int8", False))
+        if not 0.0 <= self.dropout < 1.0:
+            raise ValueError(f"dropout: 0 <= p < 1, got {self.dropout}")
+        if seg and (self.dropout or self.entropy_weight or self.int8):
+            raise ValueError("dropout, entropy_weight and int8 are for the classifiers")
         # HIP-graph capture of each fold's training step ("auto": GPU runs whose collectives, if
         # any, are on the native RCCL communicator)
         self.hip_graph = kwargs.get("hip_graph", "auto")
@@ -202,7 +214,7 @@ class Model:
                     "image_channels": self.image_channels, "loss": self.loss,
                     "optimizer": self.optimizer, "lr": self.lr, "lr_schedule": self.lr_schedule,
                     "weight_decay": self.weight_decay, "seed": self.seed,
-                    "precision": self.precision, "fp8": self.fp8}
+                    "precision": self.precision, "fp8": self.fp8, "dropout": self.dropout}
         return {"model_name": self.model_name, "weight_decay": self.weight_decay,
                 "batch_norm_decay": self.batch_norm_decay,
                 "batch_norm_epsilon": self.batch_norm_epsilon,
@@ -484,7 +496,9 @@ class Model:
         extra = ((lambda m: m.regularization_loss())
                  if self.use_regularization and hasattr(net, "regularization_loss") and
                  self.optimizer == "adam" else None)
-        trainer = self._make_trainer(net, softmax_cross_entropy, device, ctx, steps, extra)
+        loss_fn = softmax_cross_entropy if not self.entropy_weight else functools.partial(
+            confidence_penalty_cross_entropy, entropy_weight=self.entropy_weight)
+        trainer = self._make_trainer(net, loss_fn, device, ctx, steps, extra)
         start = 0
         latest = ckpt.latest_checkpoint(fold_dir)
         if latest is not None:
@@ -619,6 +633,8 @@ class Model:
             if device.type == "cuda" and self.precision != "fp32":
                 net._tdl_flat = FlatParams(net, device, lowp_dtype=torch.bfloat16, with_grad=False)
             net.eval()
+            if self.int8:
+                _models.enable_int8(net)
             labels = np.zeros(len(ids), dtype=np.int64)  # unused by the image sources
             probs = [softmax_eval(net(x), probs=True)[2].cpu() for x, _ in ClassificationPipeline(
                 src, ids, labels, batch_size, shuffle=False, repeat=False, device=device,
@@ -629,6 +645,25 @@ class Model:
         if n_models == 0:
             raise ValueError("no trained fold checkpoints found; call train first")
         return (acc / n_models).numpy()
+
+    @torch.no_grad()
+    def rank_classes(self, X, batch_size, top_k=5, labels=None):
+        """The ``top_k`` most probable classes of images ``X`` under the fold-averaged
+        probabilities of :meth:`predict_classes`: {"classes": int64 [N, k], "log_probs": float32
+        [N, k], "entropy": float32 [N]} and, with ``labels``, {"label_log_probs": float32 [N]}
+        (ops/logprob.label_log_probs on the log of the average)."""
+        if top_k > MAX_TOP_K:
+            raise ValueError(f"top_k <= {MAX_TOP_K}, got {top_k}")
+        p = torch.from_numpy(self.predict_classes(X, batch_size))
+        if self.device != "cpu" and torch.cuda.is_available():
+            p = p.cuda()
+        y = None if labels is None else torch.as_tensor(np.asarray(labels), device=p.device)
+        r = label_log_probs(p.log(), y, top_k=min(top_k, self.num_classes))
+        out = {"classes": r.top_index.cpu().numpy(), "log_probs": r.top_log_prob.cpu().numpy(),
+               "entropy": r.entropy.cpu().numpy()}
+        if y is not None:
+            out["label_log_probs"] = r.log_prob.cpu().numpy()
+        return out
 
     @torch.no_grad()
     def _evaluate(self, net, images, masks, batch, device, ctx, writer=None, step=0):

@@ -114,11 +114,34 @@ def _block_convbns(b):
     return [b.conv1, b.conv2] + ([b.conv3] if hasattr(b, "conv3") else [])
 
 
+def enable_int8(model, pointwise=False):
+    """8-bit inference (ops/int8.py) of the linear layers: in eval mode without autograd their
+    weights are quantised once per parameter version, their input rows on the fly.  Few rows (serving
+    one image) are a stream over the weights, half as long in 8 bits.  ``pointwise``: also every
+    1×1, stride-1, unpadded ConvBN, BN folded (a pass over the activations quantises them, which a
+    bf16 product does not need: half the weights' memory, not less time, at these networks'
+    sizes).  Training, evaluation with autograd and servable exports are unaffected.  Returns the
+    number of layers."""
+    from .layers import ConvBN, Linear, RowPackedConv2d, resolve_padding
+    n = 0
+    for m in model.modules():
+        if isinstance(m, Linear) and not m.conv.grad_needs_unpad():
+            m.conv.int8 = True
+            n += 1
+        elif pointwise and isinstance(m, ConvBN):
+            c = m.conv
+            if (c.k == (1, 1) and c.stride == (1, 1) and not isinstance(c, RowPackedConv2d)
+                    and tuple(resolve_padding(c.padding, 8, 8, 1, 1, c.stride, c.dilation)) == (0, 0, 0, 0)):
+                c.int8 = True
+                n += 1
+    return n
+
+
 def build(name, **kw):
     if name not in _REGISTRY:
         raise KeyError(f"unknown model {name}; have {sorted(_REGISTRY)}")
     return _REGISTRY[name](**kw)
 
 
-__all__ = ["enable_fp8", "ResNet", "resnet18", "resnet34", "resnet50", "resnet101", "resnet152",
+__all__ = ["enable_fp8", "enable_int8", "ResNet", "resnet18", "resnet34", "resnet50", "resnet101", "resnet152",
            "DeepLabResNet", "Xception41", "xception_41", "FlatParams", "build"]

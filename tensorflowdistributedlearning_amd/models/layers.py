@@ -20,7 +20,9 @@ from ..ops.pool import max_pool2d, global_avg_pool
 from ..ops.dwconv import depthwise_conv2d
 from ..ops import bnconv
 from ..ops.bnconv import DeferredBNAct, bn_act_conv
-from ..ops.common import compute_weight, flat_view
+from ..ops.common import compute_weight, export_impl, flat_view
+from ..ops.dropout import dropout, DropoutKeys
+from ..ops.int8 import Int8Weight, int8_linear
 from ..ops.fp8 import DelayedScaler, flat_weights_for, transpose_weight
 from . import params as _params
 
@@ -283,6 +285,22 @@ class Conv2d(nn.Module):
             g = ConvGeom(self.stride, pad, self.dilation)
             self._geom_cache[(H, W)] = g
         return g
+
+    int8 = False  # set by models.enable_int8: 8-bit inference of this 1×1 conv (ops/int8.py)
+
+    def int8_weight(self, w_fn, key):
+        """The :class:`ops.int8.Int8Weight` of the [Cout, 1, 1, Cin] inference weight ``w_fn()``,
+        laid out again when ``key`` (parameter version, device, …) changes."""
+        c = self.__dict__.get("_int8_w")
+        if c is None or c[0] != key:
+            w = w_fn()
+            c = self.__dict__["_int8_w"] = (key, Int8Weight.quantize(w.reshape(w.shape[0], -1).float()))
+        return c[1]
+
+    def int8_active(self):
+        """This call runs in 8 bits: enabled, inference, and not being traced for export (servable
+        programs keep the full-precision weights)."""
+        return self.int8 and not torch.is_grad_enabled() and export_impl() is None
 
     fp8 = False  # set by models.enable_fp8: e4m3 forward GEMM (ops/fp8.py)
     fp8_dgrad = False  # … and the e5m2 × e4m3 input gradient
@@ -569,6 +587,9 @@ class ConvBN(nn.Module):
         if (not self.training and into is None and not torch.is_grad_enabled()
                 and bn_fold_enabled()):
             wf, bf = self.folded_params(x.dtype, x.device)
+            if self.conv.int8_active():
+                w8 = self.conv.int8_weight(lambda: wf, (_params.version(), x.dtype, x.device))
+                return int8_linear(x, w8, bias=bf, residual=residual, relu=self.relu)
             return self.conv.forward_folded(x, wf, bf, self.relu, residual)
         if self.training:
             y, stats = self.conv(x, want_stats=True, join=join)
@@ -636,8 +657,40 @@ class Linear(nn.Module):
 
     def forward(self, x):
         N, C = x.shape
-        y = self.conv(x.reshape(N, 1, 1, C))
+        c = self.conv
+        if not self.training and c.int8_active():
+            w8 = c.int8_weight(lambda: c.weight.detach(), (_params.version(), x.device))
+            return int8_linear(x, w8, bias=None if c.bias is None else c.bias.detach().float())
+        y = c(x.reshape(N, 1, 1, C))
         return y.reshape(N, -1)
+
+
+class Dropout(nn.Module):
+    """Inverted dropout in training (ops/dropout.py: the mask is never stored).  Keys come from a
+    stream of the layer's own, made at the first training call: ``seed`` (default: drawn from
+    torch's CPU generator when the layer is built) and a call number that starts at rank · 2^40, so
+    data-parallel ranks draw different masks from one seed.  A captured step draws a new mask at
+    every replay; the stream must exist before the capture (one eager or warm-up step)."""
+
+    def __init__(self, p, seed=None):
+        super().__init__()
+        if not 0.0 <= p < 1.0:
+            raise ValueError(f"Dropout: 0 <= p < 1, got {p}")
+        self.p = float(p)
+        self.seed = int(torch.randint(0, 2 ** 62, ()).item()) if seed is None else int(seed)
+        self.__dict__["_keys"] = None
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        k = self.__dict__["_keys"]
+        if k is None or k.state.device != x.device:
+            from ..parallel.dist import get_context
+            k = self.__dict__["_keys"] = DropoutKeys(self.seed, x.device, get_context().rank << 40)
+        return dropout(x, self.p, k.next())
+
+    def extra_repr(self):
+        return f"p={self.p}"
 
 
 class DepthwiseConv2d(nn.Module):

@@ -16,7 +16,8 @@ import torch.nn as nn
 
 from ..ops import gradjoin
 
-from .layers import ConvBN, MaxPool, GlobalAvgPool, Linear, RowPackedConv2d, resolve_padding
+from .layers import (ConvBN, Dropout, MaxPool, GlobalAvgPool, Linear, RowPackedConv2d,
+                     resolve_padding)
 from ..ops.pool import bn_relu_max_pool, bn_relu_max_pool_ok
 
 
@@ -83,10 +84,11 @@ class Bottleneck(nn.Module):
 
 
 class ResNet(nn.Module):
-    """ResNet-{18,34,50,101,152}. Input NHWC [N, H, W, 3 or 8] (channels 3..7 zero)."""
+    """ResNet-{18,34,50,101,152}. Input NHWC [N, H, W, 3 or 8] (channels 3..7 zero).  ``dropout``:
+    of the pooled features before the classifier, in training."""
 
     def __init__(self, depth=50, num_classes=1000, bn_decay=0.9, bn_eps=1e-5, in_channels=3,
-                 width=64):
+                 width=64, dropout=0.0):
         super().__init__()
         kind, layers = _CFG[depth]
         block = Bottleneck if kind == "bottleneck" else BasicBlock
@@ -113,6 +115,7 @@ class ResNet(nn.Module):
         self.gap = GlobalAvgPool()
         self.num_features = cin
         self.fc = Linear(cin, num_classes) if num_classes else None
+        self.drop = Dropout(dropout) if dropout and num_classes else None
 
     @property
     def input_channels_padded(self):
@@ -140,6 +143,8 @@ class ResNet(nn.Module):
     def forward(self, x):
         x = self.forward_features(x)
         x = self.gap(x)
+        if self.drop is not None:
+            x = self.drop(x)
         if self.fc is not None:
             x = self.fc(x)
         return x

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 
 from . import params as _params
-from .layers import (ConvBN, DepthwiseConv2d, BatchNorm, GlobalAvgPool, Linear, bn_fold_enabled,
+from .layers import (ConvBN, DepthwiseConv2d, Dropout, BatchNorm, GlobalAvgPool, Linear, bn_fold_enabled,
                      fold_bn_affine)
 from ..ops import bnfold, dwfold, gradjoin
 from ..ops.dwconv import joinable
@@ -172,10 +172,10 @@ class Xception(nn.Module):
     conv+BN+ReLU) then ``stack_blocks_dense`` over ``blocks`` — a list of (scope, depth_list,
     skip_connection_type, num_units, stride, unit_rate_list, activation_fn_in_separable_conv);
     the stride of a block is in its last unit — with atrous output-stride control, and an
-    optional global-pool + logits head."""
+    optional global-pool + logits head (``dropout``: of its pooled features, in training)."""
 
     def __init__(self, blocks, num_classes=0, in_channels=3, output_stride=None, bn_decay=0.9997,
-                 bn_eps=1e-3):
+                 bn_eps=1e-3, dropout=0.0):
         super().__init__()
         bn_kw = dict(bn_decay=bn_decay, bn_eps=bn_eps)
         self.conv1_1 = ConvBN(in_channels, 32, 3, 2, _fixed_pad(3, 1), relu=True, pad_cin_to=8,
@@ -214,6 +214,7 @@ class Xception(nn.Module):
         self.num_features = cin
         self.gap = GlobalAvgPool() if num_classes else None
         self.fc = Linear(cin, num_classes) if num_classes else None
+        self.drop = Dropout(dropout) if dropout and num_classes else None
 
     def forward(self, x, return_end_points=False):
         if x.shape[-1] != self.conv1_1.conv._cin_store:
@@ -228,16 +229,17 @@ class Xception(nn.Module):
             if return_end_points:
                 ep[name] = x
         if self.fc is not None:
-            x = self.fc(self.gap(x))
+            x = self.gap(x)
+            x = self.fc(x if self.drop is None else self.drop(x))
         return (x, ep) if return_end_points else x
 
 
 class Xception41(Xception):
     def __init__(self, num_classes=1000, in_channels=3, output_stride=None, multi_grid=None,
-                 bn_decay=0.9997, bn_eps=1e-3):
+                 bn_decay=0.9997, bn_eps=1e-3, dropout=0.0):
         blocks = [b if b[5] is not None else b[:5] + (list(multi_grid or [1, 1, 1]),) + b[6:]
                   for b in XCEPTION41_BLOCKS]
-        super().__init__(blocks, num_classes, in_channels, output_stride, bn_decay, bn_eps)
+        super().__init__(blocks, num_classes, in_channels, output_stride, bn_decay, bn_eps, dropout)
 
 
 def xception_41(num_classes=1000, **kw):

@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from .common import on_gpu, ext
+from .logprob import label_log_probs
 
 
 # ----------------------------------------------------------------------------------------------
@@ -59,6 +60,17 @@ class _SoftmaxXentFn(torch.autograd.Function):
 def softmax_cross_entropy(logits, labels, label_smoothing=0.0):
     """Mean softmax cross-entropy over the batch. logits [N, K]; labels int [N]."""
     return _SoftmaxXentFn.apply(logits, labels, label_smoothing)
+
+
+def confidence_penalty_cross_entropy(logits, labels, entropy_weight=0.0, ignore_index=-100):
+    """Mean over the rows that count of −log p(label) − ``entropy_weight`` · H(p): cross-entropy
+    that rewards (> 0) or penalises (< 0) undecided rows.  ``logits`` [..., K], ``labels`` [...];
+    rows labelled ``ignore_index`` do not count (none left: 0).  One pass over the logits forward
+    and one backward (ops/logprob.py)."""
+    r = label_log_probs(logits, labels, ignore_index=ignore_index)
+    counts = (labels != ignore_index).to(r.entropy.dtype)
+    per_row = r.log_prob + entropy_weight * r.entropy * counts if entropy_weight else r.log_prob
+    return -per_row.sum() / counts.sum().clamp_min(1.0)
 
 
 def softmax_eval(logits, labels=None, probs=False):
