@@ -36,38 +36,54 @@ __device__ __forceinline__ u4v philox10(uint64_t block, uint64_t call, uint64_t 
   return u4v{c0, c1, c2, c3};
 }
 
-__device__ __forceinline__ void apply8(float* f, const u4v& r, uint32_t cut, float scale) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// E elements of a group from element `first` on: their 16 bits are in E / 2 of its words
+template <int E>
+__device__ __forceinline__ void apply(float* f, const u4v& r, int first, uint32_t cut, float scale) {
+  uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if (E == 4 && first) {
+    w[0] = w[2];
+    w[1] = w[3];
+  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < E; ++e) {
     const uint32_t h = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
     f[e] = h >= cut ? f[e] * scale : 0.f;
   }
 }
 
+// A thread's E elements are one 16-byte access: a whole group in bf16, half of one in fp32 (whose
+// other half's thread makes the same numbers again; 8 bytes per element leave time for that, and
+// 32-byte pieces per lane cost more: 22.6 M elements 41 us).
 // VEC: both pointers are 16-byte aligned; else (a view that starts inside a vector) element by element
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T* __restrict__ y,
                                                       long n, const int64_t* __restrict__ key,
                                                       uint32_t cut, float scale) {
+  constexpr int E = 16 / sizeof(T);
   const uint64_t seed = (uint64_t)key[0], call = (uint64_t)key[1];
-  const long groups = (n + 7) / 8;
-  for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < groups; g += (long)gridDim.x * 256) {
-    const long i = g * 8;
-    const bool whole = i + 8 <= n;
-    float f[8];
+  const long pieces = (n + E - 1) / E;
+  for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < pieces; g += (long)gridDim.x * 256) {
+    const long i = g * E;
+    const bool whole = i + E <= n;
+    float f[E];
     if (VEC && whole) {
-      load8(x + i, f);
+      if constexpr (E == 8) {
+        load8(x + i, f);
+      } else {
+        const float4 v = *(const float4*)(x + i);
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = i + e < n ? load1(x + i + e) : 0.f;
+      for (int e = 0; e < E; ++e) f[e] = i + e < n ? load1(x + i + e) : 0.f;
     }
-    apply8(f, philox10((uint64_t)g, call, seed), cut, scale);
+    apply<E>(f, philox10((uint64_t)(i / 8), call, seed), (int)(i % 8), cut, scale);
     if (VEC && whole) {
-      store8(y + i, f);
+      if constexpr (E == 8) store8(y + i, f);
+      else *(float4*)(y + i) = make_float4(f[0], f[1], f[2], f[3]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < E; ++e)
         if (i + e < n) store1(y + i + e, f[e]);
     }
   }
@@ -83,7 +99,7 @@ __global__ void dropout_next_key_kernel(int64_t* state, int64_t* out) {
 
 void dropout_launch(const void* x, void* y, long n, bool bf16, const int64_t* key, uint32_t cut,
                     float scale, hipStream_t st) {
-  const long blocks = ((n + 7) / 8 + 255) / 256;
+  const long e = bf16 ? 8 : 4, blocks = ((n + e - 1) / e + 255) / 256;
   const unsigned grid = (unsigned)(blocks < 256 * 16 ? blocks : 256 * 16);
   const bool vec = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
   if (bf16) {

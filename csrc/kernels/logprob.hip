@@ -171,13 +171,24 @@ __device__ __forceinline__ RowEnd row_end(const Stat& a) {
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void write_row(const LogProbArgs& a, long row, const T* x,
-                                          const RowEnd& r) {
-  if (a.labels) {
-    const long y = a.labels[row];
-    a.logp[row] = y == a.ignore ? 0.f : (y < 0 || y >= a.C) ? NAN : r.lp(load1(x + y));
+// the row's label and its logit, loaded ahead of the row (two dependent loads: behind it they would
+// end every row with their latency)
+struct RowLabel {
+  long y = 0;
+  float x = 0.f;
+  template <typename T>
+  __device__ __forceinline__ void load(const LogProbArgs& a, long row, const T* xr) {
+    if (!a.labels) return;
+    y = a.labels[row];
+    const bool in = y >= 0 && y < a.C;
+    x = load1(xr + (in ? y : 0));
+    if (!in) x = NAN;
   }
+};
+
+__device__ __forceinline__ void write_row(const LogProbArgs& a, long row, const RowLabel& l,
+                                          const RowEnd& r) {
+  if (a.labels) a.logp[row] = l.y == a.ignore ? 0.f : l.x != l.x ? NAN : r.lp(l.x);
   a.ent[row] = r.ent;
   if (a.stat) {
     a.stat[3 * row] = r.m;
@@ -233,6 +244,8 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(LogProbArgs a) {
     const bool live = row < a.N;
     const T* x = (const T*)a.x + (live ? row : 0) * a.ld;
     const int C = (int)a.C;
+    RowLabel lab;
+    if (live) lab.load(a, row, x);
     RowVec<T, LPR, V> d;
     d.load(x, C, lane, live);
     Stat st = stat_empty();
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(LogProbArgs a) {
     st.s = gsum<LPR>(st.s);
     st.t = gsum<LPR>(st.t);
     const RowEnd r = row_end(st);
-    if (live && lane == 0) write_row(a, row, x, r);
+    if (live && lane == 0) write_row(a, row, lab, r);
     if (TOPK) {
       // k times the group's maximum; NaN marks what is taken or not this lane's (maxima pass over it,
       // nothing equals it)
@@ -450,6 +463,8 @@ __global__ void __launch_bounds__(NTH) logprob_long_kernel(LogProbArgs a, int pa
     const T* x = (const T*)a.x + row * a.ld;
     const int c0 = part * part_len, c1 = (int)min((long)c0 + part_len, a.C);
     const int nvec = (c1 - c0) / 8, tail = (c1 - c0) % 8;  // the tail's elements: one per thread
+    RowLabel lab;
+    if (parts == 1) lab.load(a, row, x);
     Stat st = stat_empty();
     float vb = -INFINITY;
     int vi = tid;
@@ -571,7 +586,7 @@ __global__ void __launch_bounds__(NTH) logprob_long_kernel(LogProbArgs a, int pa
     }
     if (parts == 1) {
       const RowEnd r = row_end(st);
-      if (tid == 0) write_row(a, row, x, r);
+      if (tid == 0) write_row(a, row, lab, r);
       if (TOPK && tid < a.k) {
         a.top_lp[row * a.k + tid] = bad ? NAN : r.lp(key_val(best[tid]));
         a.top_idx[row * a.k + tid] = bad ? tid : (long)key_idx(best[tid]);
@@ -591,6 +606,8 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogProbArgs a, int par
   const int lane = threadIdx.x;
   for (long row = blockIdx.x; row < a.N; row += gridDim.x) {
     const T* x = (const T*)a.x + row * a.ld;
+    RowLabel lab;
+    lab.load(a, row, x);
     Stat st = stat_empty();
     if (lane < parts) st = ((const Stat*)a.part_stat)[row * parts + lane];
     if (TOPK) {
@@ -598,7 +615,7 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogProbArgs a, int par
       for (int i = lane; i < parts * a.k; i += 64) keys[i] = a.part_key[row * parts * a.k + i];
     }
     const RowEnd r = row_end(stat_wave(st));
-    if (lane == 0) write_row(a, row, x, r);
+    if (lane == 0) write_row(a, row, lab, r);
     if (TOPK) {
       __syncthreads();
       int at = 0;
@@ -676,11 +693,11 @@ void bwd(const LogProbGradArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// parts of 4096 classes or more while there are fewer than 512 workgroups
+// parts of 2048 classes or more while there are fewer than 512 workgroups
 int logprob_parts(long N, long C) {
   if (C <= LOGPROB_SHORT) return 1;
   long p = (512 + N - 1) / N;
-  p = p < C / 4096 ? p : C / 4096;
+  p = p < C / 2048 ? p : C / 2048;
   p = p < LOGPROB_MAX_PARTS ? p : LOGPROB_MAX_PARTS;
   return p < 1 ? 1 : (int)p;
 }
