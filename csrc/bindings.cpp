@@ -7,7 +7,6 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "kernels/kernels.h"
 #include "kernels/conv_route.h"
@@ -1093,6 +1092,12 @@ void softmax_eval(Tensor logits, c10::optional<Tensor> labels, c10::optional<Ten
 }
 
 // ------------------------------------------------------------------------- label log-probabilities
+// a launch that the driver refused (bad grid, too much LDS) is an error here, not at the next call
+void check_launch(const char* who) {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, who, ": launch failed: ", hipGetErrorString(e));
+}
+
 // rows of logits: [N, C] with unit column stride (a channel slice or padded rows are fine)
 void check_logit_rows(const Tensor& x, const char* who) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, who, ": logits [N, C] on the GPU");
@@ -1130,10 +1135,11 @@ LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& lab
   const auto f32 = x.options().dtype(torch::kFloat32);
   LogProbArgs a{};
   a.labels = opt_row_labels(labels, x, "label_log_probs");
+  const bool lab = labels.has_value() && labels->defined();  // (an empty batch has a null pointer)
   LogProbOut o;
   Tensor ps, pk;
   o.ent = torch::empty({N}, f32);
-  if (a.labels) o.logp = torch::empty({N}, f32);
+  if (lab) o.logp = torch::empty({N}, f32);
   if (k) {
     o.top_lp = torch::empty({N, k}, f32);
     o.top_idx = torch::empty({N, k}, x.options().dtype(torch::kInt64));
@@ -1153,7 +1159,7 @@ LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& lab
   a.N = N;
   a.C = C;
   a.k = (int)k;
-  a.logp = a.labels ? F32(o.logp) : nullptr;
+  a.logp = lab ? F32(o.logp) : nullptr;
   a.ent = F32(o.ent);
   if (k) {
     a.top_lp = F32(o.top_lp);
@@ -1161,7 +1167,23 @@ LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& lab
   }
   if (want_stat) a.stat = F32(o.stat);
   logprob_launch(a, !is_f32(x), parts, stream());
+  check_launch("label_log_probs");
   return o;
+}
+
+// A leaf whose gradient node belongs to an older graph that is still alive, on another stream:
+// capturing a backward pass through it would make that stream wait inside the capture, which can
+// end the process.  Refused here, where the graph can still be abandoned.
+void check_capture_leaf(const Tensor& x, const char* who) {
+  if (!x.is_leaf()) return;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream(), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(x);
+  if (!acc) return;
+  const auto s = acc->stream();
+  TORCH_CHECK(!s || *s == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().unwrap(), who,
+              ": an eager graph of this input is still alive; drop it (its outputs and losses) before "
+              "capturing a backward pass");
 }
 
 Tensor label_log_probs_bwd(Tensor x, c10::optional<Tensor> labels, Tensor stat,
@@ -1194,7 +1216,31 @@ Tensor label_log_probs_bwd(Tensor x, c10::optional<Tensor> labels, Tensor stat,
   a.C = C;
   a.dx = dx.data_ptr();
   logprob_bwd_launch(a, !is_f32(x), stream());
+  check_launch(who);
   return dx;
+}
+
+// A first derivative that was asked for with create_graph: itself, tied to what it was computed from
+// by a node that refuses to be differentiated.
+struct OnceFn : torch::autograd::Function<OnceFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& dx, const Tensor& x,
+                        const c10::optional<Tensor>& g0, const c10::optional<Tensor>& g1,
+                        const c10::optional<Tensor>& g2, std::string who) {
+    (void)x, (void)g0, (void)g1, (void)g2;
+    ctx->saved_data["who"] = std::move(who);
+    return dx;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list) {
+    TORCH_CHECK(false, ctx->saved_data["who"].toStringRef(), " is differentiable once");
+    return {};
+  }
+};
+
+Tensor once(const Tensor& dx, const Tensor& x, const torch::autograd::variable_list& g, const char* who) {
+  if (!at::GradMode::is_enabled()) return dx;
+  auto at = [&](size_t i) { return i < g.size() && g[i].defined() ? c10::optional<Tensor>(g[i]) : c10::nullopt; };
+  return OnceFn::apply(dx, x, at(0), at(1), at(2), std::string(who));
 }
 
 // The autograd node is native: one training step through the operator costs two kernel launches and
@@ -1235,12 +1281,7 @@ struct LabelLogProbsFn : torch::autograd::Function<LabelLogProbsFn> {
           rows(g[0]), g_top, g_top ? c10::optional<Tensor>(idx) : c10::nullopt,
           ctx->saved_data["ignore"].toInt()));
     }
-    if (at::GradMode::is_enabled()) {  // create_graph: an error where it is differentiated again
-      dx[0].requires_grad_(true);
-      dx = (*std::make_shared<torch::autograd::DelayedError>(
-          "label_log_probs is differentiable once", 1))(std::move(dx));
-    }
-    return {dx[0], Tensor(), Tensor(), Tensor()};
+    return {once(dx[0], x, g, "label_log_probs"), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -1248,6 +1289,7 @@ struct LabelLogProbsFn : torch::autograd::Function<LabelLogProbsFn> {
 py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int64_t ignore) {
   Tensor logp, ent, top_lp, top_idx;
   if (x.requires_grad() && at::GradMode::is_enabled()) {
+    check_capture_leaf(x, "label_log_probs");
     const auto o = LabelLogProbsFn::apply(x, labels, k, ignore);
     size_t i = 0;
     ent = o[i++];
@@ -1264,6 +1306,62 @@ py::tuple label_log_probs(Tensor x, c10::optional<Tensor> labels, int64_t k, int
   return py::make_tuple(opt(logp), ent, opt(top_lp), opt(top_idx));
 }
 
+// −mean over the rows that count of log p(label) + weight · H
+struct ConfidenceXentFn : torch::autograd::Function<ConfidenceXentFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& labels,
+                        double weight, int64_t ignore) {
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    LogProbOut o = label_log_probs_fwd(x, labels, 0, ignore, true);
+    const int64_t N = x.size(0);
+    Tensor loss = torch::empty({}, o.ent.options()), inv = torch::empty({}, o.ent.options());
+    const int64_t parts = logprob_loss_parts(N);
+    Tensor part;
+    if (parts) part = torch::empty({2 * parts}, o.ent.options().dtype(torch::kFloat64));
+    logprob_loss_launch(F32(o.logp), F32(o.ent), labels.data_ptr<int64_t>(), ignore, (float)weight, N,
+                        parts ? part.data_ptr<double>() : nullptr, F32(loss), F32(inv), stream());
+    check_launch("confidence_xent");
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["weight"] = weight;
+    ctx->save_for_backward({x, labels, o.stat, inv});
+    return loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &labels = saved[1], &stat = saved[2], &inv = saved[3];
+    torch::autograd::variable_list dx{Tensor()};
+    {
+      at::AutoGradMode off(false);
+      const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+      const Tensor dloss = g[0].to(torch::kFloat32).contiguous();
+      LogProbGradArgs a{};
+      a.x = x.data_ptr();
+      a.N = x.size(0);
+      a.C = x.size(1);
+      a.ld = a.N > 1 ? x.stride(0) : a.C;
+      a.labels = labels.data_ptr<int64_t>();
+      a.ignore = ctx->saved_data["ignore"].toInt();
+      a.stat = F32(stat);
+      a.dloss = F32(dloss);
+      a.inv_rows = F32(inv);
+      a.ent_weight = (float)ctx->saved_data["weight"].toDouble();
+      dx[0] = torch::empty({a.N, a.C}, x.options());
+      a.dx = dx[0].data_ptr();
+      if (a.N) logprob_bwd_launch(a, !is_f32(x), stream());
+      check_launch("confidence_xent backward");
+    }
+    return {once(dx[0], x, g, "confidence_penalty_cross_entropy"), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor confidence_xent(Tensor x, Tensor labels, double weight, int64_t ignore) {
+  check_logit_rows(x, "confidence_xent");
+  opt_row_labels(labels, x, "confidence_xent");
+  if (x.requires_grad() && at::GradMode::is_enabled()) check_capture_leaf(x, "confidence_xent");
+  return ConfidenceXentFn::apply(x, labels, weight, ignore);
+}
+
 // ------------------------------------------------------------------------------------------ dropout
 Tensor dropout_run(const Tensor& x0, const Tensor& key, int64_t cut) {
   const Tensor x = x0.contiguous();
@@ -1273,6 +1371,7 @@ Tensor dropout_run(const Tensor& x0, const Tensor& key, int64_t cut) {
   if (x.numel())
     dropout_launch(x.data_ptr(), y.data_ptr(), x.numel(), !is_f32(x), key.data_ptr<int64_t>(),
                    (uint32_t)cut, scale, stream());
+  check_launch("dropout");
   return y;
 }
 
@@ -1302,8 +1401,9 @@ Tensor dropout(Tensor x, Tensor key, int64_t cut) {
   TORCH_CHECK(key.scalar_type() == torch::kInt64 && key.numel() == 2 && key.is_contiguous() &&
                   key.device() == x.device(), "dropout key: contiguous int64 [2] on the input's device");
   TORCH_CHECK(cut >= 0 && cut <= 65536, "dropout: 0 <= cut <= 65536");
-  return x.requires_grad() && at::GradMode::is_enabled() ? DropoutFn::apply(x, key, cut)
-                                                         : dropout_run(x, key, cut);
+  if (!x.requires_grad() || !at::GradMode::is_enabled()) return dropout_run(x, key, cut);
+  check_capture_leaf(x, "dropout");
+  return DropoutFn::apply(x, key, cut);
 }
 
 Tensor dropout_next_key(Tensor state) {
@@ -1335,6 +1435,7 @@ std::tuple<Tensor, Tensor> int8_quantize(Tensor x) {
   if (M)
     int8_quantize_launch(x.data_ptr(), M > 1 ? x.stride(0) : K, !is_f32(x), M, K,
                          q.data_ptr<int8_t>(), F32(s), stream());
+  check_launch(who);
   return {q, s};
 }
 
@@ -1385,6 +1486,7 @@ void int8_gemm(Tensor q, Tensor qs, Tensor w, Tensor ws, int64_t K, c10::optiona
   a.qs = F32(qs);
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(y.device());
   if (a.M && a.N) int8_gemm_launch(a, !is_f32(y), stream());
+  check_launch(who);
 }
 
 // x [..., K] bf16 / fp32 -> act(x wᵀ + bias [+ res]) [..., N] in x's type
@@ -1412,13 +1514,14 @@ Tensor int8_linear(Tensor x, Tensor w, Tensor ws, int64_t N, c10::optional<Tenso
                                    relu, y2, who);
   if (!M || !N) return y;
   Tensor q, qs;
-  if (!int8_linear_fused(M, a.Kp, !is_f32(x))) {
+  if (!int8_linear_fused(M, N, a.Kp, !is_f32(x))) {
     q = torch::empty({int8_rows(M), a.Kp}, x.options().dtype(torch::kInt8));
     qs = torch::empty({M}, x.options().dtype(torch::kFloat32));
   }
   int8_linear_launch(m.data_ptr(), M > 1 ? m.stride(0) : K, K, a,
                      q.defined() ? q.data_ptr<int8_t>() : nullptr, qs.defined() ? F32(qs) : nullptr,
                      !is_f32(x), stream());
+  check_launch(who);
   return y;
 }
 
@@ -2028,6 +2131,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("probs") = py::none());
   m.def("lovasz_hinge", &lovasz_hinge);
   m.def("label_log_probs", &label_log_probs, py::arg("logits"), py::arg("labels"), py::arg("top_k"),
+        py::arg("ignore_index"));
+  m.def("confidence_xent", &confidence_xent, py::arg("logits"), py::arg("labels"), py::arg("weight"),
         py::arg("ignore_index"));
   m.def("int8_quantize", &int8_quantize, py::arg("x"));
   m.def("int8_gemm", &int8_gemm, py::arg("q"), py::arg("qs"), py::arg("w"), py::arg("ws"), py::arg("K"),

@@ -31,7 +31,7 @@ struct Int8GemmArgs {
 };
 // quantise x's rows and multiply; q / qs: room for the blocks and scales, not touched when the
 // rows are few enough to be quantised where they are used (int8_linear_fused)
-bool int8_linear_fused(long M, long Kp, bool bf16);
+bool int8_linear_fused(long M, long N, long Kp, bool bf16);
 void int8_linear_launch(const void* x, long ld, long K, const Int8GemmArgs& a, int8_t* q, float* qs,
                         bool bf16, hipStream_t st);
 void int8_gemm_launch(const Int8GemmArgs& a, bool bf16, hipStream_t st);

@@ -9,6 +9,7 @@
 #include "conv_common.h"
 #include "int8.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace tdl {
@@ -273,9 +274,9 @@ __device__ __forceinline__ void st8u(float* p, const float* f) {
 }
 
 // 16-row tiles to workgroups: XCD x takes a contiguous run (its L2 keeps what neighbours share),
-// ordered in groups of GM row tiles, down the rows first
-template <int GM>
+// ordered in groups of 8 row tiles, down the rows first
 __device__ __forceinline__ void tile_of(int id, int tm, int tn, int* m, int* n) {
+  constexpr int GM = 8;
   id = xcd_remap(id, tm * tn);
   const int per = GM * tn, g = id / per, gm = min(GM, tm - g * GM), r = id - g * per;
   *n = r / gm;
@@ -336,24 +337,24 @@ struct Tile<32, R, C> {
   }
 };
 
-// FM × FN blocks of 16 × 16 per wave, WM × WN waves, ST stages of 64 k in LDS.
+// FM × FN blocks of 16 × 16 per wave, WM × WN waves, ST stages of 64 KB k in LDS.
 //
 // Step kt: the copies of stage kt + 1 have landed (vmcnt, barrier); stage kt + ST − 1 is copied into
 // the slot of stage kt − 1, whose fragments went into products before the barrier; the fragments of
 // kt + 1 are read while the products of kt run.  Copies past the end read zeros, which keeps the
 // count of copies in flight the same in every step.
-template <typename T, int GM, int MF, int FM, int FN, int WM, int WN, int ST>
+template <typename T, int MF, int FM, int FN, int WM, int WN, int KB, int ST>
 __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   constexpr int NW = WM * WN, BM = FM * 16 * WM, BN = FN * 16 * WN;
-  constexpr int BLK = (BM + BN) / 16, PER = BLK / NW, STAGE = BLK * 1024;
-  static_assert(BLK % NW == 0, "every wave moves the same number of blocks");
+  constexpr int BLK = (BM + BN) / 16, PER = BLK * KB / NW, STAGE = BLK * KB * 1024;
+  static_assert(BLK * KB % NW == 0, "every wave moves the same number of blocks");
   static_assert(ST >= 3, "");
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nb = a.Kp / 64;
   const int tn = (a.N + BN - 1) / BN, tm = (int)((a.M + BM - 1) / BM);
   int im, in;
-  tile_of<GM>(blockIdx.x, tm, tn, &im, &in);
+  tile_of(blockIdx.x, tm, tn, &im, &in);
   const long m0 = (long)im * BM;
   const int n0 = in * BN;
   // rows past the end read as zeros: the descriptors end with the last whole block row
@@ -365,17 +366,18 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   uint32_t off[PER];
 #pragma unroll
   for (int p = 0; p < PER; ++p) {
-    const int b = p * NW + w;  // 0 .. BM/16 − 1: activations, then weights
-    off[p] = (uint32_t)((b < BM / 16 ? b : b - BM / 16) * nb) * 1024u + lane * 16u;
+    const int i = p * NW + w, b = i % BLK;  // [k block][BM/16 of activations, BN/16 of weights]
+    off[p] = (uint32_t)((b < BM / 16 ? b : b - BM / 16) * nb + i / BLK) * 1024u + lane * 16u;
   }
   auto issue = [&](int kt, int slot) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int b = p * NW + w;
-      const uint32_t o = kt < nb ? off[p] + (uint32_t)kt * 1024u : convk::OOB;
-      const uint32_t dst = base + slot * STAGE + b * 1024;
-      if ((p + 1) * NW <= BM / 16) dma_block(ra, dst, o);
-      else if (p * NW >= BM / 16) dma_block(rb, dst, o);
+      const int i = p * NW + w, b = i % BLK;
+      const uint32_t o = kt * KB + i / BLK < nb ? off[p] + (uint32_t)(kt * KB) * 1024u : convk::OOB;
+      const uint32_t dst = base + slot * STAGE + i * 1024;
+      // (which operand: known at compile time where a round of the waves does not straddle them)
+      if (p * NW % BLK + NW <= BM / 16) dma_block(ra, dst, o);
+      else if (p * NW % BLK >= BM / 16 && p * NW % BLK + NW <= BLK) dma_block(rb, dst, o);
       else dma_block(b < BM / 16 ? ra : rb, dst, o);
     }
   };
@@ -384,13 +386,17 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   const int wm = w / WN, wn = w % WN;
   const uint32_t fa0 = base + wm * FM * 1024 + Acc::lane_off(lane);
   const uint32_t fb0 = base + (BM / 16) * 1024 + wn * FN * 1024 + Acc::lane_off(lane);
-  auto frags = [&](i32x4(&fa)[FM], i32x4(&fb)[FN], int slot) {
+  auto frags = [&](i32x4(&fa)[KB][FM], i32x4(&fb)[KB][FN], int slot) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fb[j] = lds_frag(fb0 + slot * STAGE + Acc::frag_off(j));
+    for (int k = 0; k < KB; ++k) {
+      const uint32_t at = slot * STAGE + k * BLK * 1024;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fa[i] = lds_frag(fa0 + slot * STAGE + Acc::frag_off(i));
+      for (int j = 0; j < FN; ++j) fb[k][j] = lds_frag(fb0 + at + Acc::frag_off(j));
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[k][i] = lds_frag(fa0 + at + Acc::frag_off(i));
+    }
   };
-  i32x4 xa[FM], xb[FN], ya[FM], yb[FN];
+  i32x4 xa[KB][FM], xb[KB][FN], ya[KB][FM], yb[KB][FN];
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) issue(s, s);
   // Epilogue layout (below): lane l finishes 8 columns of row l / CPR of each pass.  Its scales and
@@ -434,7 +440,8 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   frags(xa, xb, 0);
   int slot = 0;  // of stage kt
   auto next = [](int s) { return s + 1 == ST ? 0 : s + 1; };
-  auto step = [&](int kt, const i32x4(&fa)[FM], const i32x4(&fb)[FN], i32x4(&ga)[FM], i32x4(&gb)[FN]) {
+  auto step = [&](int kt, const i32x4(&fa)[KB][FM], const i32x4(&fb)[KB][FN], i32x4(&ga)[KB][FM],
+                  i32x4(&gb)[KB][FN]) {
     // no product of the step before moves below the barrier: its fragments' slot is refilled here
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt<PER*(ST - 3)>();
@@ -442,10 +449,11 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
     issue(kt + ST - 1, slot == 0 ? ST - 1 : slot - 1);
     slot = next(slot);
     frags(ga, gb, slot);
-    t.products(fa, fb);
+#pragma unroll
+    for (int k = 0; k < KB; ++k) t.products(fa[k], fb[k]);
   };
-  // Kp is a multiple of 128: an even number of stages
-  for (int kt = 0; kt < nb; kt += 2) {
+  // two steps at a time; a step past the end multiplies the zeros its copies brought
+  for (int kt = 0; kt * KB < nb; kt += 2) {
     step(kt, xa, xb, ya, yb);
     step(kt + 1, ya, yb, xa, xb);
   }
@@ -524,10 +532,10 @@ void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipS
 // takes them, so the kernel is a stream over them.  A workgroup owns 16 output channels; its NW
 // waves take the blocks of 64 k in turn, U loads of 1 KiB in flight each, and add their sums in LDS.
 //
-// FUSED (x in its own type instead of quantised blocks): every workgroup quantises the few rows
-// itself, under the latency of its first weight loads.  With one to four rows that is 16 elements
-// per thread or so; a launch of its own costs more (FUSED_ROWS, FUSED_ITEMS below).
-constexpr int FUSED_ROWS = 4, FUSED_ITEMS = 4;
+// FUSED (x in its own type instead of quantised blocks): every workgroup quantises the rows itself,
+// under the latency of its first weight loads; a launch of its own costs 3 us more while that is
+// little work (1 × 2048 → 1000: 3.7 us against 7.5; int8_linear_fused below).
+constexpr int FUSED_ROWS = 16, FUSED_ITEMS = 4;
 
 template <typename T, int MB, int NW, bool FUSED>
 __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T* __restrict__ x,
@@ -633,63 +641,80 @@ __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T
   }
 }
 
-template <typename T, int GM, int MF, int FM, int FN, int WM, int WN, int ST>
+// true at the first call on each device (a kernel's LDS limit is set per device)
+struct DeviceOnce {
+  std::atomic<bool> done[64] = {};
+  bool first() {
+    int d = 0;
+    if (hipGetDevice(&d) != hipSuccess || d < 0 || d >= 64) return true;
+    return !done[d].exchange(true);
+  }
+};
+
+template <typename T, int MF, int FM, int FN, int WM, int WN, int KB, int ST>
 void run_gemm(const Int8GemmArgs& a, hipStream_t st) {
-  constexpr int BM = FM * 16 * WM, BN = FN * 16 * WN, ring = ST * (BM + BN) * 64,
+  constexpr int BM = FM * 16 * WM, BN = FN * 16 * WN, ring = ST * KB * (BM + BN) * 64,
                 epi = WM * WN * MF * (FN * 64 + 16), lds = ring > epi ? ring : epi;
-  static const bool set = hipFuncSetAttribute((const void*)gemm_kernel<T, GM, MF, FM, FN, WM, WN, ST>,
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-  (void)set;
+  static DeviceOnce once;
+  if (lds > 64 * 1024 && once.first())
+    (void)hipFuncSetAttribute((const void*)gemm_kernel<T, MF, FM, FN, WM, WN, KB, ST>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   const long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  gemm_kernel<T, GM, MF, FM, FN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, lds, st>>>(a);
+  gemm_kernel<T, MF, FM, FN, WM, WN, KB, ST><<<(unsigned)tiles, 64 * WM * WN, lds, st>>>(a);
 }
 
 template <typename T, int MB, int NW, bool FUSED>
 void run_stream(const Int8GemmArgs& a, const T* x, long ld, long K, hipStream_t st) {
   const int lds = FUSED ? (int)(a.M * a.Kp) : 0;
   if (FUSED) {
-    static const bool set = hipFuncSetAttribute((const void*)stream_kernel<T, MB, NW, FUSED>,
-                                                hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                FUSED_ITEMS * 1024 * 16) == hipSuccess;
-    (void)set;
+    static DeviceOnce once;
+    if (once.first())
+      (void)hipFuncSetAttribute((const void*)stream_kernel<T, MB, NW, FUSED>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize, FUSED_ITEMS * 1024 * 16);
   }
   stream_kernel<T, MB, NW, FUSED><<<(unsigned)((a.N + 15) / 16), 64 * NW, lds, st>>>(a, x, ld, K);
 }
 
-constexpr long STREAM_ROWS = 64;
-
 template <typename T>
 void gemm(const Int8GemmArgs& a, hipStream_t st) {
-  if (a.M <= STREAM_ROWS) {
-    const bool wide = a.Kp > 64 * 64;
+  // few rows: 32 × 2048 → 1000 3.5 us on the stream, 6.5 on tiles; 64 × 2048 → 1000 4.9 and 6.3; 64 ×
+  // 4096 → 4096 10.6 and 9.1 (each workgroup reads all the rows again: tiles share them)
+  if (a.M <= 32 || (a.M <= 64 && a.Kp <= 2048)) {
+    const bool wide = a.Kp > 64 * 64;  // waves enough to keep 4 loads or more in flight in each
     if (a.M <= 16) wide ? run_stream<T, 1, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 1, 8, false>(a, nullptr, 0, 0, st);
     else if (a.M <= 32) wide ? run_stream<T, 2, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 2, 8, false>(a, nullptr, 0, 0, st);
-    else wide ? run_stream<T, 4, 16, false>(a, nullptr, 0, 0, st) : run_stream<T, 4, 8, false>(a, nullptr, 0, 0, st);
+    else run_stream<T, 4, 8, false>(a, nullptr, 0, 0, st);
     return;
   }
   auto tiles = [&](long bm, long bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
-  // Large tiles read LDS least (8192³: 515 us, 128 × 128 tiles 582) but fill the chip late and leave
-  // one workgroup per CU, which short sums do not hide (50176 × 256 → 1024: 73 us against 55).
-  // 64 × 64 where 128 × 128 gives less than a tile to every other CU (512 × 2048 → 1000: 7.8 us
-  // against 11.0; 2049 × 1999 → 1003: 13.4 against 12.6).  The 32×32×32 form of the matrix unit
-  // needs fewer LDS reads in flight and wins on the small tiles (128 × 128: 14.3 against 19.5 us).
-  if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 8, 16, 8, 4, 2, 4, 4>(a, st);
-  else if (tiles(128, 128) >= 128) run_gemm<T, 8, 32, 4, 2, 2, 4, 4>(a, st);
-  else run_gemm<T, 8, 32, 2, 2, 2, 2, 6>(a, st);
+  // 256 × 256 reads LDS and L2 least (8192³ 515 us, 128 × 128 582; 16384 × 4096 → 1024 56 and 66) but
+  // leaves one workgroup per CU, which short sums do not hide (50176 × 256 → 1024: 73 us against 55).
+  // 64 × 64, 128 k per step, while 128 × 128 gives no more than a tile to every other CU (512 × 4096 →
+  // 4096, 128 tiles: 15.3 us against 17.7; 1024 × 4096 → 4096, 256 tiles: 28 against 21).  The 32×32×32 form of the matrix
+  // unit wins on the smaller tiles (2049 × 1999 → 1003 on 128 × 128: 14.3 us against 19.5), the
+  // 16×16×64 form on the large one (8192³: 522 against 527 us).
+  if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 16, 8, 4, 2, 4, 1, 4>(a, st);
+  else if (tiles(128, 128) > 128) run_gemm<T, 32, 4, 2, 2, 4, 1, 4>(a, st);
+  else run_gemm<T, 32, 2, 2, 2, 2, 2, 4>(a, st);
 }
 
 }  // namespace
 
-// (fp32 holds half as many items in its registers)
-bool int8_linear_fused(long M, long Kp, bool bf16) {
-  return M <= FUSED_ROWS && M * (Kp / 16) <= FUSED_ITEMS * (bf16 ? 1024 : 512);
+// Few rows, few enough 16-element items for the registers (fp32: half as many), and less than 2^20
+// (fp32: 2^19) of them over all workgroups, which all quantise the same rows: 16 × 4096 → 4096 in
+// bf16, 2^20 items, 10.2 us against 12.8 with a launch for them; 8 × 4096 → 16384, 2^21, 22.0
+// against 20.0; in fp32 8 × 4096 → 4096, 2^19, 10.6 against 14.7 and 4 × 4096 → 16384, 2^20, 26.5
+// against 22.1.
+bool int8_linear_fused(long M, long N, long Kp, bool bf16) {
+  const long items = M * (Kp / 16), all = items * ((N + 15) / 16);
+  return M <= FUSED_ROWS && items <= FUSED_ITEMS * (bf16 ? 1024 : 512) && all <= 1l << (bf16 ? 20 : 19);
 }
 
 namespace {
 
 template <typename T>
 void linear(const T* x, long ld, long K, Int8GemmArgs a, int8_t* q, float* qs, hipStream_t st) {
-  if (int8_linear_fused(a.M, a.Kp, sizeof(T) == 2)) {
+  if (int8_linear_fused(a.M, a.N, a.Kp, sizeof(T) == 2)) {
     if (a.M * (a.Kp / 16) <= FUSED_ITEMS * 512 && (a.Kp <= 64 * 64 || sizeof(T) == 4))
       return run_stream<T, 1, 8, true>(a, x, ld, K, st);
     if constexpr (sizeof(T) == 2) return run_stream<T, 1, 16, true>(a, x, ld, K, st);

@@ -463,11 +463,19 @@ struct LogProbGradArgs {
   int k;
   const float* stat;
   const float *g_logp, *g_ent, *g_top;  // null: not differentiated
+  // instead of g_logp / g_ent, the mean loss below: its gradient, 1 / rows, entropy weight
+  const float *dloss, *inv_rows;
+  float ent_weight;
   const int64_t* top_idx;
   void* dx;               // [N][C], x's type
 };
 int logprob_parts(long N, long C);  // workgroups per row the forward will use
 void logprob_launch(const LogProbArgs& a, bool bf16, int parts, hipStream_t st);
+// loss = −Σ (logp + weight · ent) / rows, inv = 1 / rows over the rows with label ≠ ignore (rows: at
+// least 1); part: 2 · logprob_loss_parts(N) doubles
+long logprob_loss_parts(long N);
+void logprob_loss_launch(const float* logp, const float* ent, const int64_t* labels, long ignore,
+                         float weight, long N, double* part, float* loss, float* inv, hipStream_t st);
 void logprob_bwd_launch(const LogProbGradArgs& a, bool bf16, hipStream_t st);
 
 // counter-based dropout (dropout.hip): y = keep ? x·scale : 0, 16 random bits per element

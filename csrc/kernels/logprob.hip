@@ -306,14 +306,20 @@ __device__ __forceinline__ RowGrad row_grad(const LogProbGradArgs& a, long row) 
   r.m = a.stat[3 * row];
   r.logs = a.stat[3 * row + 1];
   r.ent = a.stat[3 * row + 2];
-  r.h = a.g_ent ? a.g_ent[row] : 0.f;
-  r.y = a.labels && a.g_logp ? a.labels[row] : -1;
-  r.g = 0.f;
-  if (a.labels && a.g_logp && r.y != a.ignore) {
-    // a label out of range had log p = NaN: so has its gradient
-    r.g = r.y < 0 || r.y >= a.C ? NAN : a.g_logp[row];
+  const bool lab = a.labels && (a.g_logp || a.dloss);
+  r.y = lab ? a.labels[row] : -1;
+  const bool counts = !lab || r.y != a.ignore;
+  float g;
+  if (a.dloss) {  // the mean loss: every row that counts has the same factors
+    g = -a.dloss[0] * a.inv_rows[0];
+    r.h = counts ? a.ent_weight * g : 0.f;
+  } else {
+    g = a.g_logp ? a.g_logp[row] : 0.f;
+    r.h = a.g_ent ? a.g_ent[row] : 0.f;
   }
-  if (r.y == a.ignore) r.y = -1;
+  // a label out of range had log p = NaN: so has its gradient
+  r.g = !lab || !counts ? 0.f : r.y < 0 || r.y >= a.C ? NAN : g;
+  if (!counts) r.y = -1;
   const bool empty = r.logs == INFINITY;
   if (empty) r.g = r.h = 0.f;  // nothing depends on the logits
   r.gall = r.g;
@@ -387,7 +393,7 @@ constexpr int BWD_U = 2, BWD_CHUNK = 256 * 8 * BWD_U * 2;
 
 template <typename T>
 __global__ void __launch_bounds__(256) logprob_long_bwd_kernel(LogProbGradArgs a, uint32_t chunks) {
-  const uint32_t total = (uint32_t)a.N * chunks;  // < 2^32 (launcher)
+  const uint32_t total = (uint32_t)a.N * chunks;  // < 2^32: the card's memory holds fewer chunks
   const int C = (int)a.C;
   for (uint32_t b = blockIdx.x; b < total; b += gridDim.x) {
     const uint32_t r0 = b / chunks;
@@ -633,6 +639,54 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogProbArgs a, int par
   }
 }
 
+// Mean over the rows that count of −(log p + weight · H), and 1 / max(1, rows).  Several workgroups
+// leave sums in part, one workgroup adds them in order (a captured step must not clear
+// memory, and the order of float atomics would change the result).
+constexpr int LOSS_ROWS = 4096;  // rows per workgroup
+
+__global__ void __launch_bounds__(256) logprob_loss_kernel(const float* __restrict__ logp,
+                                                           const float* __restrict__ ent,
+                                                           const int64_t* __restrict__ labels,
+                                                           long ignore, float weight, long N,
+                                                           double* __restrict__ part,
+                                                           float* __restrict__ loss,
+                                                           float* __restrict__ inv) {
+  __shared__ double sh[2][256];
+  const int tid = threadIdx.x;
+  double sum = 0, rows = 0;
+  if (part && loss) {  // the join: part holds N pairs
+    for (long i = tid; i < N; i += 256) {
+      sum += part[2 * i];
+      rows += part[2 * i + 1];
+    }
+  } else {
+    const long first = (long)blockIdx.x * LOSS_ROWS, last = min(N, first + LOSS_ROWS);
+    for (long i = first + tid; i < last; i += 256)
+      if (labels[i] != ignore) {
+        sum += (double)(weight != 0.f ? fmaf(weight, ent[i], logp[i]) : logp[i]);
+        rows += 1;
+      }
+  }
+  sh[0][tid] = sum;
+  sh[1][tid] = rows;
+  for (int o = 128; o > 0; o >>= 1) {
+    __syncthreads();
+    if (tid < o) {
+      sh[0][tid] += sh[0][tid + o];
+      sh[1][tid] += sh[1][tid + o];
+    }
+  }
+  if (tid) return;
+  if (loss) {
+    const double i = 1.0 / (sh[1][0] > 1 ? sh[1][0] : 1.0);
+    *loss = (float)(-sh[0][0] * i);
+    *inv = (float)i;
+  } else {
+    part[2 * blockIdx.x] = sh[0][0];
+    part[2 * blockIdx.x + 1] = sh[1][0];
+  }
+}
+
 inline unsigned grid_for(long blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
 
 // lanes per row and vectors per lane of the short-row kernels: the fewest lanes that hold the row
@@ -708,6 +762,19 @@ void logprob_launch(const LogProbArgs& a, bool bf16, int parts, hipStream_t st) 
   parts = cdiv(a.C, part_len);
   if (bf16) fwd<bf16_t>(a, parts, part_len, st);
   else fwd<float>(a, parts, part_len, st);
+}
+
+long logprob_loss_parts(long N) { return N <= LOSS_ROWS ? 0 : (N + LOSS_ROWS - 1) / LOSS_ROWS; }
+
+void logprob_loss_launch(const float* logp, const float* ent, const int64_t* labels, long ignore,
+                         float weight, long N, double* part, float* loss, float* inv, hipStream_t st) {
+  const long parts = logprob_loss_parts(N);
+  if (!parts) {
+    logprob_loss_kernel<<<1, 256, 0, st>>>(logp, ent, labels, ignore, weight, N, nullptr, loss, inv);
+    return;
+  }
+  logprob_loss_kernel<<<(unsigned)parts, 256, 0, st>>>(logp, ent, labels, ignore, weight, N, part, nullptr, nullptr);
+  logprob_loss_kernel<<<1, 256, 0, st>>>(logp, ent, labels, ignore, weight, parts, part, loss, inv);
 }
 
 void logprob_bwd_launch(const LogProbGradArgs& a, bool bf16, hipStream_t st) {

@@ -86,6 +86,18 @@ def resolve_padding(mode, H, W, R, S, stride, dilation):
 # layers
 # ----------------------------------------------------------------------------------------------
 
+def _not_capturing(device):
+    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("8-bit weights: run the network once before capturing a graph of it")
+
+
+def _int8_weight(w):
+    """:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight.  Not inside a graph capture: its
+    replays would quantise the weight again each time."""
+    _not_capturing(w.device)
+    return Int8Weight.quantize(w.reshape(w.shape[0], -1).float())
+
+
 class FlatFlips:
     """The flipped filters (Conv2d.flip_weight) of every flat-backed conv of one flat bf16 weight
     buffer (models/params.FlatParams), refreshed by ONE launch per parameter version
@@ -287,15 +299,6 @@ class Conv2d(nn.Module):
         return g
 
     int8 = False  # set by models.enable_int8: 8-bit inference of this 1×1 conv (ops/int8.py)
-
-    def int8_weight(self, w_fn, key):
-        """The :class:`ops.int8.Int8Weight` of the [Cout, 1, 1, Cin] inference weight ``w_fn()``,
-        laid out again when ``key`` (parameter version, device, …) changes."""
-        c = self.__dict__.get("_int8_w")
-        if c is None or c[0] != key:
-            w = w_fn()
-            c = self.__dict__["_int8_w"] = (key, Int8Weight.quantize(w.reshape(w.shape[0], -1).float()))
-        return c[1]
 
     def int8_active(self):
         """This call runs in 8 bits: enabled, inference, and not being traced for export (servable
@@ -568,8 +571,21 @@ class ConvBN(nn.Module):
                 sh += conv.compute_bias().float().to(device) * s
             w = conv.compute_weight(dtype)
             wf = (w.float() * s.view(-1, 1, 1, 1)).to(dtype).contiguous()
-        self.__dict__["_fold"] = (key, wf, sh.contiguous())
+        # (the last entry: the 8-bit weight, made when it is used)
+        self.__dict__["_fold"] = (key, wf, sh.contiguous(), [])
         return wf, self.__dict__["_fold"][2]
+
+    def folded_int8(self, dtype, device):
+        """(:class:`ops.int8.Int8Weight` of the folded weight, fp32 b'): kept with the fold, so it
+        follows the moving statistics."""
+        c = self.__dict__.get("_fold")
+        if c is None or c[0] != (_params.version(), dtype, device) or not c[3]:
+            _not_capturing(device)  # before the fold: one made in a capture holds nothing yet
+        wf, bf = self.folded_params(dtype, device)
+        made = self.__dict__["_fold"][3]
+        if not made:
+            made.append(_int8_weight(wf))
+        return made[0], bf
 
     def forward(self, x, residual=None, join=None, res_join=None, into=None, defer=False):
         """``join``: gradient join for x (ops/gradjoin.py); ``res_join``: for the residual.
@@ -586,10 +602,10 @@ class ConvBN(nn.Module):
                 return self._bn_out(y, stats, residual, res_join, into, defer)
         if (not self.training and into is None and not torch.is_grad_enabled()
                 and bn_fold_enabled()):
-            wf, bf = self.folded_params(x.dtype, x.device)
             if self.conv.int8_active():
-                w8 = self.conv.int8_weight(lambda: wf, (_params.version(), x.dtype, x.device))
+                w8, bf = self.folded_int8(x.dtype, x.device)
                 return int8_linear(x, w8, bias=bf, residual=residual, relu=self.relu)
+            wf, bf = self.folded_params(x.dtype, x.device)
             return self.conv.forward_folded(x, wf, bf, self.relu, residual)
         if self.training:
             y, stats = self.conv(x, want_stats=True, join=join)
@@ -659,8 +675,11 @@ class Linear(nn.Module):
         N, C = x.shape
         c = self.conv
         if not self.training and c.int8_active():
-            w8 = c.int8_weight(lambda: c.weight.detach(), (_params.version(), x.device))
-            return int8_linear(x, w8, bias=None if c.bias is None else c.bias.detach().float())
+            key = (_params.version(), c.weight._version, x.device)
+            made = self.__dict__.get("_int8_w")
+            if made is None or made[0] != key:
+                made = self.__dict__["_int8_w"] = (key, _int8_weight(c.weight.detach()))
+            return int8_linear(x, made[1], bias=None if c.bias is None else c.bias.detach().float())
         y = c(x.reshape(N, 1, 1, C))
         return y.reshape(N, -1)
 

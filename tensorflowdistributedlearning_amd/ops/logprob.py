@@ -66,6 +66,33 @@ def ref_label_log_probs(logits, labels=None, top_k=0, ignore_index=-100, dtype=t
     return LabelLogProbs(logp, ent, tlp, ti)
 
 
+def flat_rows(logits, labels, top_k, who):
+    """Check the arguments of the log-probability operators; ``(logits [N, C] as the kernels read
+    them on the GPU, labels int64 [N] or None, leading shape)``."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{who}: logits [..., C] with C >= 1, got {tuple(logits.shape)}")
+    C = logits.shape[-1]
+    if not 0 <= top_k <= min(C, MAX_TOP_K):
+        raise ValueError(f"{who}: 0 <= top_k <= min(C, {MAX_TOP_K}), got {top_k} for {C} classes")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{who}: bf16 / fp32 logits, got {logits.dtype}")
+    lead = logits.shape[:-1]
+    if labels is not None:
+        if labels.shape != lead:
+            raise ValueError(f"{who}: labels {tuple(labels.shape)} for logits {tuple(logits.shape)}")
+        if labels.dtype.is_floating_point or labels.dtype.is_complex or labels.dtype == torch.bool:
+            raise TypeError(f"{who}: integer labels, got {labels.dtype}")
+        if labels.device != logits.device:
+            raise ValueError(f"{who}: labels on {labels.device}, logits on {logits.device}")
+        labels = labels.long()
+    if not on_gpu(logits):
+        return logits, labels, lead
+    x = logits if logits.dim() == 2 else logits.reshape(-1, C)
+    if (C > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < C):
+        x = x.contiguous()
+    return x, None if labels is None else labels.reshape(-1).contiguous(), lead
+
+
 def label_log_probs(logits, labels=None, top_k=0, ignore_index=-100):
     """Log-probability of each row's label, the entropy of its distribution and its ``top_k`` most
     probable classes.
@@ -80,30 +107,10 @@ def label_log_probs(logits, labels=None, top_k=0, ignore_index=-100):
     log-probability 0 and no gradient through it; any other label outside [0, C) gives NaN.  A row
     with a NaN or +inf gives NaN throughout and the indices 0 … top_k − 1.
     """
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"label_log_probs: logits [..., C] with C >= 1, got {tuple(logits.shape)}")
-    C = logits.shape[-1]
-    if not 0 <= top_k <= min(C, MAX_TOP_K):
-        raise ValueError(f"label_log_probs: 0 <= top_k <= min(C, {MAX_TOP_K}), got {top_k} for {C} classes")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"label_log_probs: bf16 / fp32 logits, got {logits.dtype}")
-    lead = logits.shape[:-1]
-    if labels is not None:
-        if labels.shape != lead:
-            raise ValueError(f"label_log_probs: labels {tuple(labels.shape)} for logits {tuple(logits.shape)}")
-        if labels.dtype.is_floating_point or labels.dtype.is_complex or labels.dtype == torch.bool:
-            raise TypeError(f"label_log_probs: integer labels, got {labels.dtype}")
-        if labels.device != logits.device:
-            raise ValueError(f"label_log_probs: labels on {labels.device}, logits on {logits.device}")
-        labels = labels.long()
+    x, lab, lead = flat_rows(logits, labels, top_k, "label_log_probs")
     if not on_gpu(logits):
-        return ref_label_log_probs(logits, labels, top_k, ignore_index)
-    flat = logits.dim() == 2
-    x = logits if flat else logits.reshape(-1, C)
-    if (C > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < C):
-        x = x.contiguous()
-    lab = None if labels is None else labels.reshape(-1).contiguous()
+        return ref_label_log_probs(x, lab, top_k, ignore_index)
     out = ext().label_log_probs(x, lab, int(top_k), int(ignore_index))  # with its autograd node
-    if flat:
+    if logits.dim() == 2:
         return LabelLogProbs(*out)
     return LabelLogProbs(*(None if t is None else t.reshape(lead + t.shape[1:]) for t in out))

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from .common import on_gpu, ext
-from .logprob import label_log_probs
+from .logprob import flat_rows, label_log_probs
 
 
 # ----------------------------------------------------------------------------------------------
@@ -67,10 +67,14 @@ def confidence_penalty_cross_entropy(logits, labels, entropy_weight=0.0, ignore_
     that rewards (> 0) or penalises (< 0) undecided rows.  ``logits`` [..., K], ``labels`` [...];
     rows labelled ``ignore_index`` do not count (none left: 0).  One pass over the logits forward
     and one backward (ops/logprob.py)."""
+    if on_gpu(logits):
+        x, lab, _ = flat_rows(logits, labels, 0, "confidence_penalty_cross_entropy")
+        return ext().confidence_xent(x, lab, float(entropy_weight), int(ignore_index))
     r = label_log_probs(logits, labels, ignore_index=ignore_index)
-    counts = (labels != ignore_index).to(r.entropy.dtype)
-    per_row = r.log_prob + entropy_weight * r.entropy * counts if entropy_weight else r.log_prob
-    return -per_row.sum() / counts.sum().clamp_min(1.0)
+    counts = labels != ignore_index
+    per_row = r.log_prob + entropy_weight * r.entropy if entropy_weight else r.log_prob
+    per_row = torch.where(counts, per_row, torch.zeros_like(per_row))
+    return -per_row.sum() / counts.sum().clamp_min(1)
 
 
 def softmax_eval(logits, labels=None, probs=False):

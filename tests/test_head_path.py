@@ -151,6 +151,142 @@ def test_model_options_and_ranked_classes(tmp_path):
 
 # ------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,C", [(1, 5), (7, 1000), (4096, 21), (4097, 21), (30000, 3), (65, 9000)])
+def test_gpu_confidence_penalty_loss(gpu, N, C, dtype):
+    """Loss and gradient against 64 bits.  The rows' values are within tests/test_logprob.py's bound
+    (below 2^-14 for these sizes), their mean is taken in 64 bits; a gradient entry
+    is a difference of terms of the size (|g| + |h| (1 + log C)) p."""
+    gen = torch.Generator().manual_seed(N + C)
+    x = (torch.randn(N, C, generator=gen) * 2).to(dtype)
+    y = torch.randint(0, C, (N,), generator=gen)
+    y[::5] = -100 if N > 1 else y[0]
+    for w in (0.0, 0.3):
+        xg = x.to(gpu).requires_grad_(True)
+        loss = ops.confidence_penalty_cross_entropy(xg, y.to(gpu), w)
+        g, = torch.autograd.grad(loss, xg, torch.tensor(1.7, device=gpu))
+        xd = x.double().requires_grad_(True)
+        want = ref_loss(xd, y, w)
+        gd, = torch.autograd.grad(want, xd, torch.tensor(1.7, dtype=torch.float64))
+        assert abs(float(loss.detach()) - float(want.detach())) < 2.0 ** -13
+        n = int((y != -100).sum())
+        tol = 1.7 / n * (1 + w * (1 + np.log(C))) * 2.0 ** -14 + gd.abs() * 2.0 ** -20
+        if dtype == torch.bfloat16:
+            tol = tol + gd.abs() * torch.finfo(dtype).eps / 2
+        assert bool(((g.double().cpu() - gd).abs() <= tol).all())
+        assert bool((g[y == -100] == 0).all())
+    none = ops.confidence_penalty_cross_entropy(xg, torch.full((N,), -100, device=gpu), 0.3)
+    g, = torch.autograd.grad(none, xg)
+    assert float(none.detach()) == 0.0 and bool((g == 0).all())
+
+
+@pytest.mark.gpu
+def test_gpu_loss_graph_of_many_rows(gpu):
+    """Replayed with eager work in between: nothing in the graph clears memory."""
+    x = torch.randn(3, 101, 101, 21, device=gpu, dtype=torch.bfloat16)
+    y = torch.randint(0, 21, (3, 101, 101), device=gpu)
+    xs = x.clone().requires_grad_(True)
+
+    def step():
+        loss = ops.confidence_penalty_cross_entropy(xs, y, 0.1)
+        g, = torch.autograd.grad(loss, xs)
+        return loss.detach(), g
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            xs.copy_(torch.randn_like(x) * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.gpu
+def test_gpu_autograd_refusals(gpu):
+    """Second derivatives, inputs changed in between, and a capture over a live eager graph."""
+    x = torch.randn(4, 50, device=gpu, requires_grad=True)
+    y = torch.arange(4, device=gpu)
+    for f in (lambda: ops.label_log_probs(x, y).log_prob.sum(),
+              lambda: ops.confidence_penalty_cross_entropy(x, y, 0.1)):
+        g, = torch.autograd.grad(f(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum() + x.sum(), x)  # also where another path reaches x
+        assert torch.equal(g.detach(), torch.autograd.grad(f(), x)[0])
+    z = x.detach().clone().requires_grad_(True)
+    out = ops.label_log_probs(z * 1, y).entropy.sum()
+    out.backward()  # through a non-leaf
+    assert bool(z.grad.isfinite().all())
+    v = x.detach().clone().requires_grad_(True)
+    r = ops.label_log_probs(v, y)
+    with torch.no_grad():
+        v.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.log_prob.sum().backward()
+    live = ops.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64, device=gpu)) + \
+        ops.label_log_probs(x, y).entropy[:, None]  # an eager graph of x on this stream
+    key = torch.zeros(2, dtype=torch.int64, device=gpu)
+    for f in (lambda: ops.label_log_probs(x, y), lambda: ops.dropout(x, 0.5, key),
+              lambda: ops.confidence_penalty_cross_entropy(x, y)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=gpu)
+            with pytest.raises(RuntimeError, match="eager graph of this input is still alive"):
+                f()
+    del live
+
+
+@pytest.mark.gpu
+def test_gpu_empty_and_one_dimensional_inputs(gpu):
+    y0 = torch.zeros(0, dtype=torch.long, device=gpu)
+    x0 = torch.zeros(0, 40, device=gpu, requires_grad=True)
+    r = ops.label_log_probs(x0, y0, top_k=3)
+    assert r.log_prob.shape == (0,) and r.top_index.shape == (0, 3)
+    g, = torch.autograd.grad(r.log_prob.sum(), x0)
+    assert g.shape == (0, 40)
+    assert float(ops.confidence_penalty_cross_entropy(x0, y0).detach()) == 0.0
+    v = torch.randn(40, device=gpu)
+    one = ops.label_log_probs(v, torch.tensor(3, device=gpu), top_k=2)
+    assert one.log_prob.shape == () and one.top_index.shape == (2,)
+    assert torch.equal(one.top_log_prob, ops.label_log_probs(v[None], None, top_k=2).top_log_prob[0])
+    w = ops.Int8Weight(torch.ones(6, 40, dtype=torch.int8, device=gpu), torch.ones(6, device=gpu))
+    assert ops.int8_linear(v, w).shape == (6,)
+    assert torch.equal(ops.int8_linear(v, w, residual=torch.ones(6, device=gpu)), ops.int8_linear(v, w) + 1)
+    assert ops.int8_linear(torch.zeros(0, 3, 40, device=gpu), w).shape == (0, 3, 6)
+    assert ops.quantize_rows(torch.zeros(0, 40, device=gpu)).scale.shape == (0,)
+    key = torch.zeros(2, dtype=torch.int64, device=gpu)
+    assert ops.dropout(torch.zeros(0, 3, device=gpu), 0.5, key).shape == (0, 3)
+
+
+@pytest.mark.gpu
+def test_gpu_int8_weight_follows_statistics_and_refuses_capture(gpu):
+    from tensorflowdistributedlearning_amd.models.layers import ConvBN
+    torch.manual_seed(6)
+    m = ConvBN(64, 48, 1, 1, 0, relu=True).to(gpu).eval()
+    seq = torch.nn.Sequential(m)
+    assert models.enable_int8(seq, pointwise=True) == 1
+    x = torch.randn(2, 5, 5, 64, device=gpu, dtype=torch.bfloat16)
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=gpu)
+            with pytest.raises(RuntimeError, match="before capturing"):
+                m(x)
+        a = m(x)
+        m.train()
+        m.bn.running_var.mul_(4)
+        m.eval()
+        b = m(x)
+    assert torch.allclose(b.float() * 2, a.float(), atol=0.02, rtol=0.02)
+
+
+@pytest.mark.gpu
 def test_gpu_head_training_step_and_graph(gpu):
     """Dropout → linear → entropy-regularised loss through the Trainer, eager and captured."""
     torch.manual_seed(4)
