@@ -664,7 +664,16 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LogProbArgs a, int par
     if (lane < parts) st = ((const Stat*)a.part_stat)[row * parts + lane];
     if (TOPK) {
       __syncthreads();
-      for (int i = lane; i < parts * a.k; i += 64) keys[i] = a.part_key[row * parts * a.k + i];
+      // 8 loads in flight: one after the other their latency was most of the launch
+      const unsigned long long* from = a.part_key + row * parts * a.k;
+      for (int i = lane; i < parts * a.k; i += 8 * 64) {
+        unsigned long long v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i + u * 64 < parts * a.k ? from[i + u * 64] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (i + u * 64 < parts * a.k) keys[i + u * 64] = v[u];
+      }
     }
     const RowEnd r = row_end(stat_wave(st));
     if (lane == 0) write_row(a, row, lab, r);
