@@ -473,6 +473,8 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
       t.each(i, lane, [&](int r, int c, const i32x4& v) {
         *(__attribute__((address_space(3))) i32x4*)(uintptr_t)(ep + r * PITCH + c * 4) = v;
       });
+      // lanes read what others wrote: one wave's LDS accesses run in order, and stay in it here
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int r = 0; r < MF; r += RPI) {
         const uint32_t at = ep + (r + lane / CPR) * PITCH + lane % CPR * 32;
@@ -502,6 +504,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
             if (e < left) store1(y0 + d + e, v[e]);
         }
       }
+      __builtin_amdgcn_wave_barrier();
     }
   };
   if (inside) finish(std::true_type());
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(64 * NW) stream_kernel(Int8GemmArgs a, const T
     for (int i = 0; i < FUSED_ITEMS; ++i) {
       if (i * 64 * NW >= items) break;
       uint32_t bits = d[i].top();
-      // one atomic per wave where the wave is within a row 
+      // one atomic per wave where the wave is within a row
       const int row0 = __builtin_amdgcn_readfirstlane(row[i]);
       if (__all(row[i] == row0)) {
 #pragma unroll
@@ -690,9 +693,9 @@ void gemm(const Int8GemmArgs& a, hipStream_t st) {
   // 256 × 256 reads LDS and L2 least (8192³ 515 us, 128 × 128 582; 16384 × 4096 → 1024 56 and 66) but
   // leaves one workgroup per CU, which short sums do not hide (50176 × 256 → 1024: 73 us against 55).
   // 64 × 64, 128 k per step, while 128 × 128 gives no more than a tile to every other CU (512 × 4096 →
-  // 4096, 128 tiles: 15.3 us against 17.7; 1024 × 4096 → 4096, 256 tiles: 28 against 21).  The 32×32×32 form of the matrix
-  // unit wins on the smaller tiles (2049 × 1999 → 1003 on 128 × 128: 14.3 us against 19.5), the
-  // 16×16×64 form on the large one (8192³: 522 against 527 us).
+  // 4096, 128 tiles: 15.3 us against 17.7; 1024 × 4096 → 4096, 256 tiles: 28 against 21).  The
+  // 32×32×32 form of the matrix unit wins on the smaller tiles (2049 × 1999 → 1003 on 128 × 128: 14.3
+  // us against 19.5), the 16×16×64 form on the large one (8192³: 522 against 527 us).
   if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 16, 8, 4, 2, 4, 1, 4>(a, st);
   else if (tiles(128, 128) > 128) run_gemm<T, 32, 4, 2, 2, 4, 1, 4>(a, st);
   else run_gemm<T, 32, 2, 2, 2, 2, 2, 4>(a, st);

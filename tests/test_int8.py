@@ -158,7 +158,8 @@ def test_gpu_quantize_extremes_and_views(gpu):
 SHAPES = [(1, 1, 1), (1, 2048, 1000), (2, 64, 16), (4, 100, 33), (5, 8192, 257), (15, 333, 70),
           (16, 128, 128), (17, 1000, 1003), (31, 65, 4), (33, 64, 65), (64, 512, 1000), (65, 2048, 96),
           (127, 129, 127), (128, 128, 256), (129, 640, 129), (300, 1999, 301), (513, 256, 1024),
-          (1000, 64, 64), (2049, 1999, 1003), (4000, 130, 17), (1, 131071, 3), (260, 20000, 40)]
+          (1000, 64, 64), (2049, 1999, 1003), (4000, 130, 17), (1, 131071, 3), (260, 20000, 40), (16, 4096, 50), (16, 4100, 50),
+          (7, 9000, 20), (48, 5000, 100), (40, 2000, 33), (900, 1100, 3000), (4700, 1100, 2600)]
 
 
 @pytest.mark.gpu
@@ -251,3 +252,16 @@ def test_gpu_graph_replays_and_side_stream(gpu, M):
         want = ops.int8_linear(x, w, bias)
         torch.cuda.synchronize()
         assert all(torch.equal(out, want) for _, out in graphs)
+
+
+@pytest.mark.gpu
+def test_gpu_outputs_past_32_bit_offsets(gpu):
+    """More than 2^32 outputs: the last rows equal a small product of the same rows."""
+    M, K, N = 70000, 65, 65537
+    x, wq, ws, bias, _ = make(M, K, 1, torch.bfloat16, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    wq = torch.randint(-127, 128, (N, K), generator=g, device=gpu, dtype=torch.int8)
+    w = ops.Int8Weight(wq, torch.rand(N, generator=g, device=gpu))
+    y = ops.int8_linear(x, w)
+    for a in (0, M // 2, M - 40):
+        assert torch.equal(y[a:a + 40], ops.int8_linear(x[a:a + 40].contiguous(), w))

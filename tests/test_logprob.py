@@ -308,3 +308,24 @@ def test_gpu_graph_replays_and_side_stream(gpu):
         torch.cuda.synchronize()
         for _, out in graphs:
             assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,C", [(70000, 65537), (4300000, 1001)])
+def test_gpu_offsets_past_32_bits(gpu, N, C):
+    """More than 2^32 logits: rows at both ends equal the same rows alone."""
+    x = torch.zeros(N, C, device=gpu, dtype=torch.bfloat16)
+    for a in (0, N - 50):
+        x[a:a + 50] = torch.randn(50, C, device=gpu).to(torch.bfloat16)
+    y = torch.arange(N, device=gpu) * 7 % C
+    x.requires_grad_(True)
+    r = ops.label_log_probs(x, y, top_k=3)
+    d, = torch.autograd.grad(r.log_prob, x, torch.ones(N, device=gpu))
+    for a in (0, N - 50):
+        part = x.detach()[a:a + 50].clone().requires_grad_(True)
+        q = ops.label_log_probs(part, y[a:a + 50], top_k=3)
+        e, = torch.autograd.grad(q.log_prob, part, torch.ones(50, device=gpu))
+        # (few rows are split over workgroups: another order of additions)
+        assert torch.allclose(r.log_prob[a:a + 50], q.log_prob, rtol=0, atol=2 * tol_rows(C))
+        assert torch.equal(r.top_index[a:a + 50], q.top_index)
+        assert torch.allclose(d[a:a + 50].float(), e.float(), rtol=2.0 ** -7, atol=1e-6)
