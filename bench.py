@@ -254,6 +254,8 @@ def main():
     def step():
         tr.train_step(x, y)
 
+    if args.int8 and args.mode != "infer":
+        raise SystemExit("--int8: with --mode infer")
     if args.mode == "infer":
         if bc.dtype == "fp8":
             raise SystemExit("--mode infer: bf16 / fp32")

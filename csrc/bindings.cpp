@@ -7,6 +7,7 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include "kernels/kernels.h"
 #include "kernels/conv_route.h"
@@ -1102,7 +1103,7 @@ void check_launch(const char* who) {
 void check_logit_rows(const Tensor& x, const char* who) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, who, ": logits [N, C] on the GPU");
   TORCH_CHECK(x.scalar_type() == torch::kBFloat16 || is_f32(x), who, ": bf16 / fp32 logits");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (int64_t(1) << 31) - 64, who, ": 1 <= classes < 2^31 - 64");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= LOGPROB_MAX_C, who, ": 1 <= classes <= ", LOGPROB_MAX_C);
   TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, who, ": classes must be contiguous");
   TORCH_CHECK(x.size(0) <= 1 || x.stride(0) >= x.size(1), who, ": rows must not overlap");
 }
@@ -1173,13 +1174,20 @@ LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& lab
 
 // A leaf whose gradient node belongs to an older graph that is still alive, on another stream:
 // capturing a backward pass through it would make that stream wait inside the capture, which can
-// end the process.  Refused here, where the graph can still be abandoned.
+// end the process.  Refused here, where the graph can still be abandoned.  x may be the leaf itself or
+// reshapes and copies of it (nodes of one input).
 void check_capture_leaf(const Tensor& x, const char* who) {
-  if (!x.is_leaf()) return;
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream(), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
-  const auto acc = torch::autograd::impl::try_get_grad_accumulator(x);
-  if (!acc) return;
+  std::shared_ptr<torch::autograd::Node> acc;
+  if (x.is_leaf()) {
+    acc = torch::autograd::impl::try_get_grad_accumulator(x);
+  } else {
+    acc = x.grad_fn();
+    while (acc && acc->num_outputs() == 1) acc = acc->next_edge(0).function;
+  }
+  if (!dynamic_cast<torch::autograd::AccumulateGrad*>(acc.get())) return;
   const auto s = acc->stream();
   TORCH_CHECK(!s || *s == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().unwrap(), who,
               ": an eager graph of this input is still alive; drop it (its outputs and losses) before "

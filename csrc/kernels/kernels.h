@@ -440,12 +440,13 @@ void upsample_bwd_launch(const float* dy, float* dx, const int* ih, const float*
 constexpr int LOGPROB_SHORT = 2048;   // longest row that stays in one wave's registers
 constexpr int LOGPROB_MAX_PARTS = 64;
 constexpr int LOGPROB_MAX_K = 32;
+constexpr long LOGPROB_MAX_C = (1l << 31) - (1l << 16);  // a step past a row's end is still an int
 struct LogProbArgs {
   const void* x;
   long ld;
   const int64_t* labels;  // null: no log-probabilities
   long ignore;
-  long N, C;              // C < 2^31 − 64
+  long N, C;              // C ≤ LOGPROB_MAX_C
   int k;                  // ≤ min(C, LOGPROB_MAX_K)
   float *logp, *ent;      // [N]
   float* top_lp;          // [N][k]

@@ -504,6 +504,8 @@ class Model:
         if latest is not None:
             start = ckpt.restore(latest, net, trainer.optimizer, trainer.flat)
             trainer.global_step = start
+            if getattr(net, "drop", None) is not None:
+                net.drop.start_at(start)  # one mask per step
             if ctx.is_distributed:
                 trainer.broadcast_state()
         stepper = _Stepper(trainer, self._use_graph(device, ctx))
@@ -652,8 +654,8 @@ class Model:
         probabilities of :meth:`predict_classes`: {"classes": int64 [N, k], "log_probs": float32
         [N, k], "entropy": float32 [N]} and, with ``labels``, {"label_log_probs": float32 [N]}
         (ops/logprob.label_log_probs on the log of the average)."""
-        if top_k > MAX_TOP_K:
-            raise ValueError(f"top_k <= {MAX_TOP_K}, got {top_k}")
+        if not 1 <= top_k <= MAX_TOP_K:
+            raise ValueError(f"1 <= top_k <= {MAX_TOP_K}, got {top_k}")
         p = torch.from_numpy(self.predict_classes(X, batch_size))
         if self.device != "cpu" and torch.cuda.is_available():
             p = p.cuda()

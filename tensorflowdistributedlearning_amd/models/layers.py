@@ -91,11 +91,21 @@ def _not_capturing(device):
         raise RuntimeError("8-bit weights: run the network once before capturing a graph of it")
 
 
-def _int8_weight(w):
-    """:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight.  Not inside a graph capture: its
-    replays would quantise the weight again each time."""
+def _int8_weight(w, old=None):
+    """:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight, written into ``old`` where that fits
+    (graphs captured with it go on to read the new values).  Not inside a graph capture: its replays
+    would quantise the weight again each time.  Done when it returns: the next call may be on
+    another stream."""
     _not_capturing(w.device)
-    return Int8Weight.quantize(w.reshape(w.shape[0], -1).float())
+    with torch.inference_mode(False), torch.no_grad():
+        new = Int8Weight.quantize(w.reshape(w.shape[0], -1).float())
+        if old is not None and (old.n, old.k, old.device) == (new.n, new.k, new.device):
+            old.blocks.copy_(new.blocks)
+            old.scale.copy_(new.scale)
+            new = old
+    if w.is_cuda:
+        torch.cuda.current_stream(w.device).synchronize()
+    return new
 
 
 class FlatFlips:
@@ -584,7 +594,8 @@ class ConvBN(nn.Module):
         wf, bf = self.folded_params(dtype, device)
         made = self.__dict__["_fold"][3]
         if not made:
-            made.append(_int8_weight(wf))
+            self.__dict__["_int8_w"] = _int8_weight(wf, self.__dict__.get("_int8_w"))
+            made.append(self.__dict__["_int8_w"])
         return made[0], bf
 
     def forward(self, x, residual=None, join=None, res_join=None, into=None, defer=False):
@@ -675,11 +686,13 @@ class Linear(nn.Module):
         N, C = x.shape
         c = self.conv
         if not self.training and c.int8_active():
-            key = (_params.version(), c.weight._version, x.device)
-            made = self.__dict__.get("_int8_w")
-            if made is None or made[0] != key:
-                made = self.__dict__["_int8_w"] = (key, _int8_weight(c.weight.detach()))
-            return int8_linear(x, made[1], bias=None if c.bias is None else c.bias.detach().float())
+            w = c.weight
+            key = (_params.version(), None if w.is_inference() else w._version)
+            made = self.__dict__.get("_int8_w")  # (key, the parameter, its 8-bit form)
+            if made is None or made[0] != key or made[1] is not w or made[2].device != w.device:
+                q = _int8_weight(w.detach(), made and made[2])
+                made = self.__dict__["_int8_w"] = (key, w, q)
+            return int8_linear(x, made[2], bias=None if c.bias is None else c.bias.detach().float())
         y = c(x.reshape(N, 1, 1, C))
         return y.reshape(N, -1)
 
@@ -689,7 +702,8 @@ class Dropout(nn.Module):
     stream of the layer's own, made at the first training call: ``seed`` (default: drawn from
     torch's CPU generator when the layer is built) and a call number that starts at rank · 2^40, so
     data-parallel ranks draw different masks from one seed.  A captured step draws a new mask at
-    every replay; the stream must exist before the capture (one eager or warm-up step)."""
+    every replay; the stream must exist before the capture (one eager or warm-up step).
+    ``start_at(n)``: the next call is number n (a resumed run draws what the whole run would)."""
 
     def __init__(self, p, seed=None):
         super().__init__()
@@ -697,6 +711,11 @@ class Dropout(nn.Module):
             raise ValueError(f"Dropout: 0 <= p < 1, got {p}")
         self.p = float(p)
         self.seed = int(torch.randint(0, 2 ** 62, ()).item()) if seed is None else int(seed)
+        self.first = 0
+        self.__dict__["_keys"] = None
+
+    def start_at(self, n):
+        self.first = int(n)
         self.__dict__["_keys"] = None
 
     def forward(self, x):
@@ -705,7 +724,8 @@ class Dropout(nn.Module):
         k = self.__dict__["_keys"]
         if k is None or k.state.device != x.device:
             from ..parallel.dist import get_context
-            k = self.__dict__["_keys"] = DropoutKeys(self.seed, x.device, get_context().rank << 40)
+            k = self.__dict__["_keys"] = DropoutKeys(self.seed, x.device,
+                                                     (get_context().rank << 40) + self.first)
         return dropout(x, self.p, k.next())
 
     def extra_repr(self):

@@ -18,6 +18,7 @@ import torch
 from .common import on_gpu, ext
 
 MAX_TOP_K = 32  # csrc/kernels/kernels.h LOGPROB_MAX_K
+MAX_CLASSES = 2 ** 31 - 2 ** 16  # LOGPROB_MAX_C: the kernels count inside a row in 32 bits
 
 
 class LabelLogProbs(NamedTuple):
@@ -72,6 +73,8 @@ def flat_rows(logits, labels, top_k, who):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{who}: logits [..., C] with C >= 1, got {tuple(logits.shape)}")
     C = logits.shape[-1]
+    if C > MAX_CLASSES:
+        raise ValueError(f"{who}: at most {MAX_CLASSES} classes, got {C}")
     if not 0 <= top_k <= min(C, MAX_TOP_K):
         raise ValueError(f"{who}: 0 <= top_k <= min(C, {MAX_TOP_K}), got {top_k} for {C} classes")
     if logits.dtype not in (torch.bfloat16, torch.float32):

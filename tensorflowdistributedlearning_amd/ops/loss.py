@@ -67,6 +67,8 @@ def confidence_penalty_cross_entropy(logits, labels, entropy_weight=0.0, ignore_
     that rewards (> 0) or penalises (< 0) undecided rows.  ``logits`` [..., K], ``labels`` [...];
     rows labelled ``ignore_index`` do not count (none left: 0).  One pass over the logits forward
     and one backward (ops/logprob.py)."""
+    if labels is None:
+        raise ValueError("confidence_penalty_cross_entropy: labels [...] are required")
     if on_gpu(logits):
         x, lab, _ = flat_rows(logits, labels, 0, "confidence_penalty_cross_entropy")
         return ext().confidence_xent(x, lab, float(entropy_weight), int(ignore_index))

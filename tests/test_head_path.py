@@ -149,6 +149,39 @@ def test_model_options_and_ranked_classes(tmp_path):
         m.rank_classes(6, 4, top_k=33)
 
 
+def test_resumed_run_draws_the_same_masks(tmp_path):
+    from tensorflowdistributedlearning_amd.model import Model
+    kw = dict(n_gpus=1, n_fold=4, arch="resnet18", image_size=32, num_classes=10, synthetic=True,
+              device="cpu", save_best=0, export_format="none", max_folds=1, dropout=0.5, lr=0.05,
+              lr_schedule="step", lr_decay_steps=3, lr_decay_rate=0.5, save_checkpoints_steps=2)
+    whole = Model(str(tmp_path / "a"), "none", **kw).train(64, None, batch_size=8, steps=4)[0]
+    Model(str(tmp_path / "b"), "none", **kw).train(64, None, batch_size=8, steps=2)
+    rest = Model(str(tmp_path / "b"), "none", **kw).train(64, None, batch_size=8, steps=4)[0]
+    np.testing.assert_allclose(rest["train_loss"], whole["train_loss"][2:], rtol=1e-4, atol=1e-5)
+    m = Model(str(tmp_path / "b"), "none", **kw)
+    for k in (0, -1):
+        with pytest.raises(ValueError, match="top_k"):
+            m.rank_classes(4, 4, top_k=k)
+
+
+def test_int8_linear_follows_its_parameter():
+    torch.manual_seed(8)
+    m = Linear(40, 6).eval()
+    models.enable_int8(m)
+    x = torch.randn(3, 40)
+    with torch.inference_mode():
+        a = m(x)
+    blocks = m.__dict__["_int8_w"][2].blocks
+    with torch.no_grad():
+        m.conv.weight.mul_(-1)
+        b = m(x)
+        assert m.__dict__["_int8_w"][2].blocks is blocks  # written in place
+        m.conv.weight = torch.nn.Parameter(-m.conv.weight.detach())  # version 0 like the first one
+        c = m(x)
+    bias = m.conv.bias.detach()
+    assert torch.allclose(b - bias, bias - a, atol=1e-6) and torch.equal(c, a)
+
+
 # ------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -353,3 +386,54 @@ def test_gpu_int8_serving_path(gpu, pointwise):
             torch.cuda.synchronize()
             assert torch.equal(out.top_index, want.top_index)
             assert torch.equal(out.top_log_prob, want.top_log_prob)
+
+
+@pytest.mark.gpu
+def test_gpu_capture_refusal_sees_through_reshapes(gpu):
+    """Logits of more than two dimensions reach the kernels as a view of the leaf."""
+    x = torch.randn(2, 3, 50, device=gpu, requires_grad=True)
+    t = torch.randn(3, 50, 4, device=gpu, requires_grad=True)
+    y = torch.zeros(2, 3, dtype=torch.long, device=gpu)
+    z = torch.zeros(3, 4, dtype=torch.long, device=gpu)
+    live = x.sum() + t.sum()
+    for f in (lambda: ops.label_log_probs(x, y), lambda: ops.confidence_penalty_cross_entropy(x, y),
+              lambda: ops.label_log_probs(t.transpose(1, 2), z)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=gpu)
+            with pytest.raises(RuntimeError, match="eager graph of this input is still alive"):
+                f()
+    del live
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # without one it is captured
+        g, = torch.autograd.grad(ops.label_log_probs(x, y).log_prob.sum(), x)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want, = torch.autograd.grad(ops.label_log_probs(x, y).log_prob.sum(), x)
+        assert torch.equal(g, want)
+
+
+@pytest.mark.gpu
+def test_gpu_int8_graph_follows_the_weights(gpu):
+    """A captured forward reads the 8-bit weights of the last eager call, on whichever stream."""
+    from tensorflowdistributedlearning_amd.models import params
+    torch.manual_seed(7)
+    m = Linear(256, 48).to(gpu).eval()
+    models.enable_int8(m)
+    x = torch.randn(5, 256, device=gpu, dtype=torch.bfloat16)
+    with torch.no_grad():
+        m(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        for i in range(3):
+            m.conv.weight.mul_(-1.5)
+            params.bump_version()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(torch.cuda.Stream()):
+                want = m(x)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)

@@ -5,6 +5,7 @@ Tolerances.  A row's sums are chains of at most L = C / 256 + 32 additions of te
 size, at most (1 + log C) s).  log p adds the rounding of x − m and of the final difference."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -329,3 +330,29 @@ def test_gpu_offsets_past_32_bits(gpu, N, C):
         assert torch.allclose(r.log_prob[a:a + 50], q.log_prob, rtol=0, atol=2 * tol_rows(C))
         assert torch.equal(r.top_index[a:a + 50], q.top_index)
         assert torch.allclose(d[a:a + 50].float(), e.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_refuses_rows_past_the_kernels_counters():
+    """Shapes only (stride 0): nothing of that size is read."""
+    x = torch.zeros(1).expand(1, 2 ** 31 - 100)
+    for f in (lambda: ops.label_log_probs(x, torch.zeros(1, dtype=torch.long)),
+              lambda: ops.confidence_penalty_cross_entropy(x, torch.zeros(1, dtype=torch.long))):
+        with pytest.raises(ValueError, match="classes"):
+            f()
+
+
+@pytest.mark.gpu
+def test_gpu_longest_row(gpu):
+    """Equal logits: s = C exactly (C = 32767 * 2^16), so log p = -log C to one rounding of each of
+    log s and its difference, H = log C, and the gradient is 1 - 1/C at the label, -1/C elsewhere."""
+    C = 2 ** 31 - 2 ** 16
+    x = torch.zeros(1, C, device=gpu, dtype=torch.bfloat16, requires_grad=True)
+    r = ops.label_log_probs(x, torch.tensor([C - 1], device=gpu), top_k=3)
+    want = float(np.log(float(C)))
+    for got in (-r.log_prob, r.entropy, -r.top_log_prob[:, 2]):
+        assert abs(float(got.detach()) - want) <= want * 2.0 ** -22
+    assert r.top_index.tolist() == [[0, 1, 2]]
+    d, = torch.autograd.grad(r.log_prob, x)
+    assert float(d[0, C - 1]) == 1.0
+    lo, hi = float(d[0, :C - 1].min()), float(d[0, :C - 1].max())
+    assert lo == hi and abs(lo * C + 1) <= 2.0 ** -8 + 2.0 ** -17  # bf16; exp of a log to 2^-22 x 22
