@@ -139,62 +139,68 @@ __device__ __forceinline__ uint32_t quant4(const float* f, const RowScale& r) {
                                0x05040100u);
 }
 
-// A workgroup of NW waves quantises 16 rows.  Lane l of a wave holds 16 elements of row l % 16 at
-// k = 64 b + 16 (l / 16): reads are 16 segments of 128 bytes, the write is one block of 1 KiB.
-// Wave w takes blocks w, w + NW, …; V of them stay in registers, longer rows are read twice.
-template <typename T, int NW, int V, bool LONG>
+// A workgroup of NW waves quantises RG rows (16 or 4).  Lane l of a wave holds 16 elements of row
+// l % RG at k = (1024 / RG) u + 16 (l / RG).  RG = 16: reads are 16 segments of 64 elements, the write
+// is one block of 1 KiB; RG = 4: 4 segments of 256 elements and 16 pieces of 64 bytes of 4 blocks.
+// Wave w takes steps u = w, w + NW, …; V of them stay in registers, longer rows are read twice.
+template <typename T, int RG, int NW, int V, bool LONG>
 __global__ void __launch_bounds__(64 * NW) quantize_kernel(const T* __restrict__ x, long ld, long M,
                                                            long K, int nb, int8_t* __restrict__ q,
                                                            float* __restrict__ scale) {
-  __shared__ uint32_t sh[NW][16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
-  const long groups = (M + 15) / 16;
+  constexpr int BW = 16 / RG;  // blocks of 64 k a wave covers at once
+  __shared__ uint32_t sh[NW][RG];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane % RG, c = lane / RG;
+  const int nu = (nb + BW - 1) / BW;
+  const long groups = (M + 15) / 16 * BW;
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
-    const long row = g * 16 + r;
+    const long row = g * RG + r;
     const bool live = row < M;
     const T* xr = x + (live ? row : 0) * ld;
     Raw16<T> d[V];
     uint32_t bits = 0;
-    auto fetch = [&](Raw16<T>& raw, int b) {
-      const long k = (long)b * 64 + c * 16;
+    auto fetch = [&](Raw16<T>& raw, int u) {
+      const long k = ((long)u * (64 / RG) + c) * 16;
       raw.load(xr + k, live ? K - k : 0);
     };
-    for (int b0 = w; b0 < nb; b0 += NW * V) {
+    for (int u0 = w; u0 < nu; u0 += NW * V) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (b0 + v * NW < nb) fetch(d[v], b0 + v * NW);
+        if (u0 + v * NW < nu) fetch(d[v], u0 + v * NW);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (b0 + v * NW < nb) bits = max(bits, d[v].top());
+        if (u0 + v * NW < nu) bits = max(bits, d[v].top());
       if (!LONG) break;
     }
-    bits = max(bits, __shfl_xor(bits, 16, 64));
-    bits = max(bits, __shfl_xor(bits, 32, 64));
+#pragma unroll
+    for (int o = RG; o < 64; o *= 2) bits = max(bits, __shfl_xor(bits, o, 64));
     __syncthreads();
-    if (lane < 16) sh[w][lane] = bits;
+    if (lane < RG) sh[w][lane] = bits;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NW; ++i) bits = max(bits, sh[i][r]);
     // a NaN or an infinity makes the row's scale NaN: it cannot be held in 8 bits
     const bool bad = bits >= INF_BITS;
     const float top = fmaxf(__uint_as_float(bits), TINY);
-    if (threadIdx.x < 16 && live) scale[row] = bad ? NAN : top / 127.f;
+    if (threadIdx.x < RG && live) scale[row] = bad ? NAN : top / 127.f;
     const RowScale rs = row_scale(top);
-    auto emit = [&](const Raw16<T>& raw, int b) {
+    auto emit = [&](const Raw16<T>& raw, int u) {
       float f[16];
       raw.get(f);
       uint32_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = bad ? 0u : quant4<T>(f + 4 * i, rs);
-      *(uint4*)(q + (g * nb + b) * 1024 + lane * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+      const int b = u * BW + c / 4;
+      if (BW == 1 || b < nb)
+        *(uint4*)(q + (row / 16 * nb + b) * 1024 + (c % 4 * 16 + row % 16) * 16) =
+            make_uint4(o[0], o[1], o[2], o[3]);
     };
-    for (int b0 = w; b0 < nb; b0 += NW * V) {
+    for (int u0 = w; u0 < nu; u0 += NW * V) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (LONG && b0 + v * NW < nb) fetch(d[v], b0 + v * NW);
+        if (LONG && u0 + v * NW < nu) fetch(d[v], u0 + v * NW);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (b0 + v * NW < nb) emit(d[v], b0 + v * NW);
+        if (u0 + v * NW < nu) emit(d[v], u0 + v * NW);
       if (!LONG) break;
     }
   }
@@ -264,9 +270,17 @@ __device__ __forceinline__ void ld8u(const float* p, float* f) {
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
+// two values per conversion instruction
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void st8u(bf16_t* p, const float* f) {
-  const uint4 v = pack8(f);
-  *(q4_a2*)p = q4_a2{v.x, v.y, v.z, v.w};
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bf16x2 h = __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), bf16x2);
+    w[i] = __builtin_bit_cast(uint32_t, h);
+  }
+  *(q4_a2*)p = q4_a2{w[0], w[1], w[2], w[3]};
 }
 __device__ __forceinline__ void st8u(float* p, const float* f) {
   ((q4_a4*)p)[0] = q4_a4{f[0], f[1], f[2], f[3]};
@@ -343,8 +357,9 @@ struct Tile<32, R, C> {
 // the slot of stage kt − 1, whose fragments went into products before the barrier; the fragments of
 // kt + 1 are read while the products of kt run.  Copies past the end read zeros, which keeps the
 // count of copies in flight the same in every step.
+// (16 waves per CU, two workgroups, where the accumulators leave registers for it)
 template <typename T, int MF, int FM, int FN, int WM, int WN, int KB, int ST>
-__global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
+__global__ void __launch_bounds__(64 * WM * WN, FM * FN <= 8 ? 4 : 2) gemm_kernel(Int8GemmArgs a) {
   constexpr int NW = WM * WN, BM = FM * 16 * WM, BN = FN * 16 * WN;
   constexpr int BLK = (BM + BN) / 16, PER = BLK * KB / NW, STAGE = BLK * KB * 1024;
   static_assert(BLK * KB % NW == 0, "every wave moves the same number of blocks");
@@ -401,9 +416,10 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   for (int s = 0; s < ST - 1; ++s) issue(s, s);
   // Epilogue layout (below): lane l finishes 8 columns of row l / CPR of each pass.  Its scales and
   // biases are loaded behind the first copies (one after the other behind the products they cost
-  // more than a short sum), and on small tiles the residual, for which large ones have no registers.
+  // more than a short sum), and the residual where it leaves registers for two workgroups per CU
+  // (50176 × 256 → 1024 fp32: 94 us, loaded ahead there too 105).
   constexpr int CPR = FN * 2, RPI = 64 / CPR, PASSES = FM * 16 / RPI;
-  constexpr bool PRE = PASSES * 8 * sizeof(T) <= 128;
+  constexpr bool PRE = PASSES * 8 * sizeof(T) <= 64;
   const bool inside = m0 + BM <= a.M && n0 + BN <= a.N;
   const int col = n0 + wn * FN * 16 + lane % CPR * 8;
   const int left = a.N - col;
@@ -494,7 +510,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
         }
         if (a.relu) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays NaN
+          for (int e = 0; e < 8; ++e) v[e] = __builtin_elementwise_maximum(v[e], 0.f);  // NaN stays NaN
         }
         if (W || left >= 8) {
           st8u(y0 + d, v);
@@ -511,23 +527,32 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_kernel(Int8GemmArgs a) {
   else finish(std::false_type());
 }
 
-template <typename T>
-void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipStream_t st) {
-  const int nb = (int)(int8_kp(K) / 64);
-  const long groups = (M + 15) / 16;
+template <typename T, int RG>
+void quantize_groups(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipStream_t st) {
+  const int nb = (int)(int8_kp(K) / 64), nu = (nb * RG + 15) / 16;
+  const long groups = (M + 15) / 16 * (16 / RG);
   const unsigned grid = (unsigned)(groups < (1 << 20) ? groups : (1 << 20));
   // waves enough that each holds few blocks: 16 rows alone are little work for a workgroup
 #define QUANT(NW, V, LONG)                                                                      \
-  return quantize_kernel<T, NW, V, LONG><<<grid, 64 * NW, 0, st>>>(x, ld, M, K, nb, q, scale)
-  if (nb <= 4) QUANT(4, 1, false);
-  if (nb <= 8) QUANT(8, 1, false);
-  if (nb <= 16) QUANT(16, 1, false);
-  if (nb <= 32) QUANT(16, 2, false);
-  if (nb <= 64) QUANT(16, 4, false);
+  return quantize_kernel<T, RG, NW, V, LONG><<<grid, 64 * NW, 0, st>>>(x, ld, M, K, nb, q, scale)
+  if (nu <= 4) QUANT(4, 1, false);
+  if (nu <= 8) QUANT(8, 1, false);
+  if (nu <= 16) QUANT(16, 1, false);
+  if (nu <= 32) QUANT(16, 2, false);
+  if (nu <= 64) QUANT(16, 4, false);
   if constexpr (sizeof(T) == 2)  // (fp32: more registers than there are)
-    if (nb <= 128) QUANT(16, 8, false);
+    if (nu <= 128) QUANT(16, 8, false);
   QUANT(16, 4, true);
 #undef QUANT
+}
+template <typename T>
+void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipStream_t st) {
+  // 4 rows per workgroup where 16 would leave CUs idle (256 × 4096 bf16: 4.2 us against 8.2; 4096 ×
+  // 4096: 12.2 against 10.6, whose 64-byte pieces of the blocks cost more) or hold too much of a row
+  // per wave (8192 × 8192: 33.5 against 42.2; 1024 × 8192 fp32 10.1 against 36.9)
+  const long few = sizeof(T) == 2 ? 160 * 16 : 96 * 16;
+  if (K > 4096 || (K > 512 && M < few)) quantize_groups<T, 4>(x, ld, M, K, q, scale, st);
+  else quantize_groups<T, 16>(x, ld, M, K, q, scale, st);
 }
 
 // ------------------------------------------------------------------------------- few rows

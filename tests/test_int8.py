@@ -265,3 +265,20 @@ def test_gpu_outputs_past_32_bit_offsets(gpu):
     y = ops.int8_linear(x, w)
     for a in (0, M // 2, M - 40):
         assert torch.equal(y[a:a + 40], ops.int8_linear(x[a:a + 40].contiguous(), w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(1535, 600), (1536, 600), (2559, 600), (2561, 600), (50, 512), (50, 513),
+                                 (30, 4097), (2600, 5000), (21, 16385), (9, 33000)])
+def test_gpu_quantize_row_groups(gpu, M, K, dtype):
+    """Where the quantiser changes the rows of a workgroup and what it holds of a row; the padding
+    rows of the last group are written too."""
+    x = make(M, K, 1, dtype, seed=M + K)[0]
+    x[M - 1, K // 2] = float("inf")
+    r = ops.quantize_rows(x.to(gpu))
+    q, s = ref_quantize_rows(x)
+    assert torch.equal(from_blocks(r.blocks, M, K).cpu(), q)
+    assert torch.equal(r.scale[:-1].cpu(), s[:-1]) and bool(r.scale[-1].isnan())
+    full = from_blocks(r.blocks, *r.blocks.shape).cpu()
+    assert int(full[M:].abs().sum()) == 0 and int(full[:, K:].abs().sum()) == 0
