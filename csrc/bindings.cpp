@@ -1179,7 +1179,11 @@ LogProbOut label_log_probs_fwd(const Tensor& x, const c10::optional<Tensor>& lab
 void check_capture_leaf(const Tensor& x, const char* who) {
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream(), &st) != hipSuccess || st == hipStreamCaptureStatusNone) return;
+  if (hipStreamIsCapturing(stream(), &st) != hipSuccess) {
+    (void)hipGetLastError();  // the default stream, beside another thread's capture: not this call's error
+    return;
+  }
+  if (st == hipStreamCaptureStatusNone) return;
   std::shared_ptr<torch::autograd::Node> acc;
   if (x.is_leaf()) {
     acc = torch::autograd::impl::try_get_grad_accumulator(x);
