@@ -91,21 +91,25 @@ def _not_capturing(device):
         raise RuntimeError("8-bit weights: run the network once before capturing a graph of it")
 
 
-def _int8_weight(w, old=None):
-    """:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight, written into ``old`` where that fits
-    (graphs captured with it go on to read the new values).  Not inside a graph capture: its replays
-    would quantise the weight again each time.  Done when it returns: the next call may be on
-    another stream."""
+def _int8_weight(w, bias=None, old=None):
+    """(:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight, copy of ``bias`` or None), written
+    into the pair ``old`` where that fits: a graph captured with it goes on to read the new values,
+    all of one call.  Not inside a graph capture: its replays would quantise the weight again each
+    time.  Done when it returns: the next call may be on another stream."""
     _not_capturing(w.device)
     with torch.inference_mode(False), torch.no_grad():
         new = Int8Weight.quantize(w.reshape(w.shape[0], -1).float())
-        if old is not None and (old.n, old.k, old.device) == (new.n, new.k, new.device):
-            old.blocks.copy_(new.blocks)
-            old.scale.copy_(new.scale)
-            new = old
+        if old is not None and (old[0].n, old[0].k, old[0].device) == (new.n, new.k, new.device):
+            old[0].blocks.copy_(new.blocks)
+            old[0].scale.copy_(new.scale)
+            if bias is not None:
+                old[1].copy_(bias)
+            pair = old
+        else:
+            pair = (new, None if bias is None else bias.clone())
     if w.is_cuda:
         torch.cuda.current_stream(w.device).synchronize()
-    return new
+    return pair
 
 
 class FlatFlips:
@@ -581,22 +585,25 @@ class ConvBN(nn.Module):
                 sh += conv.compute_bias().float().to(device) * s
             w = conv.compute_weight(dtype)
             wf = (w.float() * s.view(-1, 1, 1, 1)).to(dtype).contiguous()
-        # (the last entry: the 8-bit weight, made when it is used)
+        # (the last entry: the 8-bit weight and its bias, made when they are used)
         self.__dict__["_fold"] = (key, wf, sh.contiguous(), [])
         return wf, self.__dict__["_fold"][2]
 
     def folded_int8(self, dtype, device):
-        """(:class:`ops.int8.Int8Weight` of the folded weight, fp32 b'): kept with the fold, so it
-        follows the moving statistics."""
+        """(:class:`ops.int8.Int8Weight` of the folded weight, fp32 b'): made once per fold, so they
+        follow the moving statistics, in the same storage every time (one per compute type and
+        device)."""
+        key = (dtype, device)
         c = self.__dict__.get("_fold")
-        if c is None or c[0] != (_params.version(), dtype, device) or not c[3]:
+        if c is None or c[0] != (_params.version(), *key) or not c[3]:
             _not_capturing(device)  # before the fold: one made in a capture holds nothing yet
         wf, bf = self.folded_params(dtype, device)
         made = self.__dict__["_fold"][3]
         if not made:
-            self.__dict__["_int8_w"] = _int8_weight(wf, self.__dict__.get("_int8_w"))
-            made.append(self.__dict__["_int8_w"])
-        return made[0], bf
+            kept = self.__dict__.setdefault("_int8_w", {})
+            kept[key] = _int8_weight(wf, bf, kept.get(key))
+            made.append(kept[key])
+        return made[0]
 
     def forward(self, x, residual=None, join=None, res_join=None, into=None, defer=False):
         """``join``: gradient join for x (ops/gradjoin.py); ``res_join``: for the residual.
@@ -690,7 +697,7 @@ class Linear(nn.Module):
             key = (_params.version(), None if w.is_inference() else w._version)
             made = self.__dict__.get("_int8_w")  # (key, the parameter, its 8-bit form)
             if made is None or made[0] != key or made[1] is not w or made[2].device != w.device:
-                q = _int8_weight(w.detach(), made and made[2])
+                q, _ = _int8_weight(w.detach(), old=made and (made[2], None))
                 made = self.__dict__["_int8_w"] = (key, w, q)
             return int8_linear(x, made[2], bias=None if c.bias is None else c.bias.detach().float())
         y = c(x.reshape(N, 1, 1, C))

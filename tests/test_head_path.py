@@ -437,3 +437,58 @@ def test_gpu_int8_graph_follows_the_weights(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+def _refolded(m, i):
+    """New statistics, affine parameters and weights, as a training phase leaves them."""
+    m.train()
+    with torch.no_grad():
+        m.bn.running_mean.add_(0.5 + i)
+        m.bn.running_var.mul_(2.0)
+        m.bn.beta.add_(0.25)
+        m.conv.weight.mul_(-1.5)
+    m.eval()
+
+
+def test_int8_pointwise_refresh_is_in_place():
+    """Weight, scales and folded bias keep their storage over a refold: a graph reads all three."""
+    from tensorflowdistributedlearning_amd.models.layers import ConvBN
+    torch.manual_seed(9)
+    m = ConvBN(24, 10, 1, 1, 0, relu=True).eval()
+    assert models.enable_int8(torch.nn.Sequential(m), pointwise=True) == 1
+    x = torch.randn(2, 3, 3, 24)
+    with torch.no_grad():
+        m(x)
+        w, b = m.folded_int8(x.dtype, x.device)
+        where = [t.data_ptr() for t in (w.blocks, w.scale, b)]
+        for i in range(2):
+            _refolded(m, i)
+            y = m(x)
+            w2, b2 = m.folded_int8(x.dtype, x.device)
+            assert [t.data_ptr() for t in (w2.blocks, w2.scale, b2)] == where
+            wf, bf = m.folded_params(x.dtype, x.device)
+            assert torch.equal(b2, bf)
+            fresh = ops.int8_linear(x, ops.Int8Weight.quantize(wf.view(10, 24)), bias=bf, relu=True)
+            assert torch.equal(y, fresh)
+
+
+@pytest.mark.gpu
+def test_gpu_int8_pointwise_graph_follows_the_fold(gpu):
+    """A captured 8-bit ConvBN reads weight, scales and bias of the last eager call."""
+    from tensorflowdistributedlearning_amd.models.layers import ConvBN
+    torch.manual_seed(10)
+    m = ConvBN(64, 48, 1, 1, 0, relu=True).to(gpu).eval()
+    models.enable_int8(torch.nn.Sequential(m), pointwise=True)
+    x = torch.randn(2, 5, 5, 64, device=gpu, dtype=torch.bfloat16)
+    with torch.no_grad():
+        old = m(x).clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        for i in range(3):
+            _refolded(m, i)
+            want = m(x)
+            torch.full((64, 48), 1e9, device=gpu)  # storage that was released has other contents
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and not torch.equal(out, old)
