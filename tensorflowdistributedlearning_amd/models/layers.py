@@ -8,6 +8,7 @@ batch_norm / max_pool2d / separable_conv2d under resnet_arg_scope, core/resnet.p
 from __future__ import annotations
 
 import math
+import threading
 
 import torch
 import torch.nn as nn
@@ -85,6 +86,9 @@ def resolve_padding(mode, H, W, R, S, stride, dilation):
 # ----------------------------------------------------------------------------------------------
 # layers
 # ----------------------------------------------------------------------------------------------
+
+_int8_lock = threading.RLock()  # over "is the 8-bit form out of date" and its refresh
+
 
 def _not_capturing(device):
     if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
@@ -594,16 +598,21 @@ class ConvBN(nn.Module):
         follow the moving statistics, in the same storage every time (one per compute type and
         device)."""
         key = (dtype, device)
-        c = self.__dict__.get("_fold")
-        if c is None or c[0] != (_params.version(), *key) or not c[3]:
+
+        def current():
+            c = self.__dict__.get("_fold")
+            return c[3][0] if c is not None and c[0] == (_params.version(), *key) and c[3] else None
+        made = current()
+        if made is None:
             _not_capturing(device)  # before the fold: one made in a capture holds nothing yet
-        wf, bf = self.folded_params(dtype, device)
-        made = self.__dict__["_fold"][3]
-        if not made:
-            kept = self.__dict__.setdefault("_int8_w", {})
-            kept[key] = _int8_weight(wf, bf, kept.get(key))
-            made.append(kept[key])
-        return made[0]
+            with _int8_lock:
+                made = current()
+                if made is None:
+                    wf, bf = self.folded_params(dtype, device)
+                    kept = self.__dict__.setdefault("_int8_w", {})
+                    made = kept[key] = _int8_weight(wf, bf, kept.get(key))
+                    self.__dict__["_fold"][3].append(made)
+        return made
 
     def forward(self, x, residual=None, join=None, res_join=None, into=None, defer=False):
         """``join``: gradient join for x (ops/gradjoin.py); ``res_join``: for the residual.
@@ -693,15 +702,25 @@ class Linear(nn.Module):
         N, C = x.shape
         c = self.conv
         if not self.training and c.int8_active():
-            w = c.weight
-            key = (_params.version(), None if w.is_inference() else w._version)
-            made = self.__dict__.get("_int8_w")  # (key, the parameter, its 8-bit form)
-            if made is None or made[0] != key or made[1] is not w or made[2].device != w.device:
-                q, _ = _int8_weight(w.detach(), old=made and (made[2], None))
-                made = self.__dict__["_int8_w"] = (key, w, q)
-            return int8_linear(x, made[2], bias=None if c.bias is None else c.bias.detach().float())
+            return int8_linear(x, self._int8(c.weight),
+                               bias=None if c.bias is None else c.bias.detach().float())
         y = c(x.reshape(N, 1, 1, C))
         return y.reshape(N, -1)
+
+    def _int8(self, w):
+        """The 8-bit form of parameter ``w`` as it is now."""
+        key = (_params.version(), None if w.is_inference() else w._version)
+
+        def current():
+            made = self.__dict__.get("_int8_w")  # (key, the parameter, its 8-bit form)
+            return made and made[0] == key and made[1] is w and made[2].device == w.device
+        if not current():
+            with _int8_lock:
+                if not current():
+                    old = self.__dict__.get("_int8_w")
+                    q, _ = _int8_weight(w.detach(), old=old and (old[2], None))
+                    self.__dict__["_int8_w"] = (key, w, q)
+        return self.__dict__["_int8_w"][2]
 
 
 class Dropout(nn.Module):

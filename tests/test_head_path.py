@@ -1,6 +1,7 @@
 """The classification head's operators as the models use them: dropout before the classifier,
 the entropy-regularised loss, 8-bit linear layers in inference, ranked predictions."""
 import copy
+import time
 
 import numpy as np
 import pytest
@@ -492,3 +493,36 @@ def test_gpu_int8_pointwise_graph_follows_the_fold(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want) and not torch.equal(out, old)
+
+
+def test_int8_weight_is_made_once_by_two_threads(monkeypatch):
+    """Two threads that both find the 8-bit form out of date get the same one: a graph captured with
+    either's follows later refreshes."""
+    import threading
+    from tensorflowdistributedlearning_amd.models import layers
+    from tensorflowdistributedlearning_amd.models.layers import ConvBN
+    calls, quantize = [], ops.Int8Weight.quantize
+
+    def slow(w):
+        calls.append(1)
+        time.sleep(0.2)
+        return quantize(w)
+    monkeypatch.setattr(layers.Int8Weight, "quantize", staticmethod(slow))
+    lin, bn = Linear(40, 6).eval(), ConvBN(40, 6, 1, 1, 0).eval()
+    models.enable_int8(torch.nn.Sequential(lin, bn), pointwise=True)
+    for m, x in ((lin, torch.randn(3, 40)), (bn, torch.randn(1, 3, 1, 40))):
+        calls.clear()
+        seen = []
+        real = layers.int8_linear
+        monkeypatch.setattr(layers, "int8_linear", lambda a, w, **k: (seen.append(w), real(a, w, **k))[1])
+
+        def work():
+            with torch.no_grad():
+                m(x)
+        ts = [threading.Thread(target=work) for _ in range(2)]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+        monkeypatch.setattr(layers, "int8_linear", real)
+        assert len(calls) == 1 and len(seen) == 2 and seen[0] is seen[1]
