@@ -98,12 +98,17 @@ def _not_capturing(device):
 def _int8_weight(w, bias=None, old=None):
     """(:class:`ops.int8.Int8Weight` of a [Cout, 1, 1, Cin] weight, copy of ``bias`` or None), written
     into the pair ``old`` where that fits: a graph captured with it goes on to read the new values,
-    all of one call.  Not inside a graph capture: its replays would quantise the weight again each
-    time.  Done when it returns: the next call may be on another stream."""
+    all of one call.  What any stream of the device has queued before the refresh still reads the old
+    ones; a replay that another thread launches while it runs may read some of each, so such threads
+    keep their replays away from calls that follow a change of parameters.  Not inside a graph
+    capture: its replays would quantise the weight again each time.  Done when it returns: the next
+    call may be on another stream."""
     _not_capturing(w.device)
     with torch.inference_mode(False), torch.no_grad():
         new = Int8Weight.quantize(w.reshape(w.shape[0], -1).float())
         if old is not None and (old[0].n, old[0].k, old[0].device) == (new.n, new.k, new.device):
+            if w.is_cuda:
+                torch.cuda.synchronize(w.device)  # earlier products and replays, on whichever stream
             old[0].blocks.copy_(new.blocks)
             old[0].scale.copy_(new.scale)
             if bias is not None:

@@ -526,3 +526,38 @@ def test_int8_weight_is_made_once_by_two_threads(monkeypatch):
             t.join()
         monkeypatch.setattr(layers, "int8_linear", real)
         assert len(calls) == 1 and len(seen) == 2 and seen[0] is seen[1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["linear", "pointwise"])
+def test_gpu_int8_refresh_waits_for_earlier_products(gpu, kind):
+    """A product, and a replay, that another stream has queued but not run read the weights of
+    their call, not those of a refresh issued after them."""
+    from tensorflowdistributedlearning_amd.models import params
+    from tensorflowdistributedlearning_amd.models.layers import ConvBN
+    torch.manual_seed(11)
+    m = (Linear(1024, 512) if kind == "linear" else ConvBN(1024, 512, 1, 1, 0)).to(gpu).eval()
+    assert models.enable_int8(torch.nn.Sequential(m), pointwise=True) == 1
+    x = torch.randn(300, 1024, device=gpu, dtype=torch.bfloat16)
+    if kind == "pointwise":
+        x = x.view(3, 10, 10, 1024)
+    with torch.no_grad():
+        want = m(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        for replay in (False, True):
+            torch.cuda.synchronize()
+            a = torch.cuda.Stream()
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(20_000_000)  # the refresh below is issued before this ends
+                if replay:
+                    graph.replay()
+                else:
+                    got = m(x)
+            m.conv.weight.mul_(-1.5)
+            params.bump_version()
+            new = m(x)
+            torch.cuda.synchronize()
+            assert torch.equal(out if replay else got, want) and not torch.equal(new, want)
+            want = new
