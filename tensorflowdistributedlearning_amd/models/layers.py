@@ -734,7 +734,11 @@ class Dropout(nn.Module):
     torch's CPU generator when the layer is built) and a call number that starts at rank · 2^40, so
     data-parallel ranks draw different masks from one seed.  A captured step draws a new mask at
     every replay; the stream must exist before the capture (one eager or warm-up step).
-    ``start_at(n)``: the next call is number n (a resumed run draws what the whole run would)."""
+    ``start_at(n)``: the next call is number n (a resumed run draws what the whole run would).
+
+    Every call draws its own mask, also the one that activation recomputation makes in the backward
+    pass, so without a key the layer refuses to run there.  With ``key`` (one :meth:`next_key`, drawn
+    outside the recomputed function and passed through it) it is a function of its arguments."""
 
     def __init__(self, p, seed=None):
         super().__init__()
@@ -749,15 +753,28 @@ class Dropout(nn.Module):
         self.first = int(n)
         self.__dict__["_keys"] = None
 
-    def forward(self, x):
+    def next_key(self, device):
+        """The key of the next call, drawn from the layer's stream on ``device``."""
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        k = self.__dict__["_keys"]
+        if k is None or k.state.device != device:
+            from ..parallel.dist import get_context
+            k = self.__dict__["_keys"] = DropoutKeys(self.seed, device,
+                                                     (get_context().rank << 40) + self.first)
+        return k.next()
+
+    def forward(self, x, key=None):
         if not self.training or self.p == 0.0:
             return x
-        k = self.__dict__["_keys"]
-        if k is None or k.state.device != x.device:
-            from ..parallel.dist import get_context
-            k = self.__dict__["_keys"] = DropoutKeys(self.seed, x.device,
-                                                     (get_context().rank << 40) + self.first)
-        return dropout(x, self.p, k.next())
+        if key is None:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("Dropout: called inside a backward pass (activation recomputation), where it "
+                                   "draws a new mask, not the forward's: draw key = layer.next_key(device) "
+                                   "outside the recomputed function and pass it in, layer(x, key=key)")
+            key = self.next_key(x.device)
+        return dropout(x, self.p, key)
 
     def extra_repr(self):
         return f"p={self.p}"

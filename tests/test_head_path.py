@@ -561,3 +561,27 @@ def test_gpu_int8_refresh_waits_for_earlier_products(gpu, kind):
             torch.cuda.synchronize()
             assert torch.equal(out if replay else got, want) and not torch.equal(new, want)
             want = new
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_dropout_layer_under_recomputation(reentrant, device):
+    """Activation recomputation calls the layer again in the backward pass: without a key it would
+    draw another mask than the forward's (refused); with one it is a function of its arguments."""
+    from torch.utils.checkpoint import checkpoint
+    d = Dropout(0.5, seed=4)
+    x = torch.ones(64, 32, device=device, requires_grad=True)
+    y = checkpoint(lambda t: d(t * 2) ** 2, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="draws a new mask"):
+        y.sum().backward()
+    d.eval()
+    checkpoint(lambda t: d(t * 2) ** 2, x, use_reentrant=reentrant).sum().backward()  # no mask
+    d.train()
+    x.grad = None
+    key = d.next_key(device)
+    y = checkpoint(lambda t, k: d(t * 2, key=k) ** 2, x, key, use_reentrant=reentrant)
+    y.sum().backward()
+    keep = ref_dropout_keep(2048, 0.5, key.cpu()).view(64, 32)
+    # y = (2 · 2 x)² = 16 where kept, its derivative 2 · 4 x · 4 = 32: exact in fp32
+    assert torch.equal(y.detach().cpu(), keep * 16.0) and torch.equal(x.grad.cpu(), keep * 32.0)
+    assert torch.equal(d.eval()(x, key=key), x)
