@@ -734,7 +734,8 @@ class Dropout(nn.Module):
     torch's CPU generator when the layer is built) and a call number that starts at rank · 2^40, so
     data-parallel ranks draw different masks from one seed.  A captured step draws a new mask at
     every replay; the stream must exist before the capture (one eager or warm-up step).
-    ``start_at(n)``: the next call is number n (a resumed run draws what the whole run would).
+    ``start_at(n)``: the next call is number n, captured steps included (a resumed run draws what the
+    whole run would).  Each device has a stream of its own, with the same numbers.
 
     Every call draws its own mask, also the one that activation recomputation makes in the backward
     pass, so without a key the layer refuses to run there.  With ``key`` (one :meth:`next_key`, drawn
@@ -747,11 +748,17 @@ class Dropout(nn.Module):
         self.p = float(p)
         self.seed = int(torch.randint(0, 2 ** 62, ()).item()) if seed is None else int(seed)
         self.first = 0
-        self.__dict__["_keys"] = None
+        self.__dict__["_streams"] = {}  # by device; kept: captured steps go on drawing from them
+        self.__dict__["_keys"] = None   # the one in use
+
+    def _first(self):
+        from ..parallel.dist import get_context
+        return (get_context().rank << 40) + self.first
 
     def start_at(self, n):
         self.first = int(n)
-        self.__dict__["_keys"] = None
+        for k in self.__dict__["_streams"].values():
+            k.start_at(self._first())
 
     def next_key(self, device):
         """The key of the next call, drawn from the layer's stream on ``device``."""
@@ -760,9 +767,10 @@ class Dropout(nn.Module):
             device = torch.device("cuda", torch.cuda.current_device())
         k = self.__dict__["_keys"]
         if k is None or k.state.device != device:
-            from ..parallel.dist import get_context
-            k = self.__dict__["_keys"] = DropoutKeys(self.seed, device,
-                                                     (get_context().rank << 40) + self.first)
+            streams = self.__dict__["_streams"]
+            if device not in streams:
+                streams[device] = DropoutKeys(self.seed, device, self._first())
+            k = self.__dict__["_keys"] = streams[device]
         return k.next()
 
     def forward(self, x, key=None):

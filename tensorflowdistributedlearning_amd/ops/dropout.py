@@ -98,6 +98,18 @@ class DropoutKeys:
             raise RuntimeError("DropoutKeys: make it (run one step) before capturing a graph")
         self.state = torch.tensor([seed, first], dtype=torch.int64).to(device)
 
+    def start_at(self, first):
+        """The next key is (seed, first), in steps captured with this stream too: the state is
+        written where it is, behind every draw that is queued on the device."""
+        cuda = self.state.device.type == "cuda"
+        if cuda:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("DropoutKeys.start_at: not inside a graph capture")
+            torch.cuda.synchronize(self.state.device)
+        self.state[1] = first
+        if cuda:
+            torch.cuda.current_stream(self.state.device).synchronize()
+
     def next(self):
         if on_gpu(self.state):
             return ext().dropout_next_key(self.state)

@@ -585,3 +585,37 @@ def test_dropout_layer_under_recomputation(reentrant, device):
     # y = (2 · 2 x)² = 16 where kept, its derivative 2 · 4 x · 4 = 32: exact in fp32
     assert torch.equal(y.detach().cpu(), keep * 16.0) and torch.equal(x.grad.cpu(), keep * 32.0)
     assert torch.equal(d.eval()(x, key=key), x)
+
+
+def test_dropout_stream_outlives_start_at_and_other_devices():
+    """A captured step advances the stream's state at every replay: the state stays where it is for
+    as long as the layer lives."""
+    d, x, y = Dropout(0.5, seed=3), torch.ones(64), torch.ones(64, device="meta")
+    d(x)
+    state = d.__dict__["_keys"].state
+    d.start_at(7)
+    assert torch.equal(d(x) != 0, ref_dropout_keep(64, 0.5, torch.tensor([3, 7])))
+    assert d.__dict__["_keys"].state is state and int(state[1]) == 8
+    d(y)  # another device in between: neither stream starts again
+    assert torch.equal(d(x) != 0, ref_dropout_keep(64, 0.5, torch.tensor([3, 8])))
+    assert d.__dict__["_keys"].state is state
+    early = Dropout(0.5, seed=3)
+    early.start_at(8)
+    assert torch.equal(early(x) != 0, ref_dropout_keep(64, 0.5, torch.tensor([3, 8])))
+
+
+@pytest.mark.gpu
+def test_gpu_dropout_start_at_reaches_a_captured_step(gpu):
+    d = Dropout(0.5, seed=5)
+    x = torch.ones(5000, device=gpu)
+    d(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = d(x)
+    for first in (20, 3):
+        d.start_at(first)
+        for i in range(3):
+            torch.full((2,), -1, dtype=torch.int64, device=gpu)  # storage that was released
+            graph.replay()
+            keep = ref_dropout_keep(5000, 0.5, torch.tensor([5, first + i]))
+            assert torch.equal(out.cpu() != 0, keep)
