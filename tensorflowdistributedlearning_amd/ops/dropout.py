@@ -96,7 +96,8 @@ class DropoutKeys:
         if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             # a state made inside the graph would be made again by every replay: the same masks
             raise RuntimeError("DropoutKeys: make it (run one step) before capturing a graph")
-        self.state = torch.tensor([seed, first], dtype=torch.int64).to(device)
+        with torch.inference_mode(False):  # an ordinary tensor, whichever call comes first
+            self.state = torch.tensor([seed, first], dtype=torch.int64).to(device)
 
     def start_at(self, first):
         """The next key is (seed, first), in steps captured with this stream too: the state is

@@ -604,6 +604,14 @@ def test_dropout_stream_outlives_start_at_and_other_devices():
     assert torch.equal(early(x) != 0, ref_dropout_keep(64, 0.5, torch.tensor([3, 8])))
 
 
+def test_dropout_stream_made_under_inference_mode():
+    d, x = Dropout(0.5, seed=3), torch.ones(64, requires_grad=True)
+    with torch.inference_mode():
+        d(x)
+    d(x).sum().backward()
+    assert torch.equal(x.grad != 0, ref_dropout_keep(64, 0.5, torch.tensor([3, 1])))
+
+
 @pytest.mark.gpu
 def test_gpu_dropout_start_at_reaches_a_captured_step(gpu):
     d = Dropout(0.5, seed=5)
