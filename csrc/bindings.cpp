@@ -1099,6 +1099,11 @@ void check_launch(const char* who) {
   TORCH_CHECK(e == hipSuccess, who, ": launch failed: ", hipGetErrorString(e));
 }
 
+// The kernels carry no tangents: a dual tensor's would be lost without a word.
+void check_no_tangent(const Tensor& t, const char* who) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, ": no forward-mode derivative on the GPU");
+}
+
 // rows of logits: [N, C] with unit column stride (a channel slice or padded rows are fine)
 void check_logit_rows(const Tensor& x, const char* who) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, who, ": logits [N, C] on the GPU");
@@ -1106,6 +1111,7 @@ void check_logit_rows(const Tensor& x, const char* who) {
   TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= LOGPROB_MAX_C, who, ": 1 <= classes <= ", LOGPROB_MAX_C);
   TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, who, ": classes must be contiguous");
   TORCH_CHECK(x.size(0) <= 1 || x.stride(0) >= x.size(1), who, ": rows must not overlap");
+  check_no_tangent(x, who);
 }
 
 const int64_t* opt_row_labels(const c10::optional<Tensor>& t, const Tensor& x, const char* who) {
@@ -1280,6 +1286,7 @@ struct LabelLogProbsFn : torch::autograd::Function<LabelLogProbsFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &labels = saved[1], &stat = saved[2], &idx = saved[3];
     auto rows = [](const Tensor& t) {
+      check_no_tangent(t, "label_log_probs backward");
       return t.defined() ? c10::optional<Tensor>(t.to(torch::kFloat32).contiguous()) : c10::nullopt;
     };
     const bool lab = labels.defined();
@@ -1346,6 +1353,7 @@ struct ConfidenceXentFn : torch::autograd::Function<ConfidenceXentFn> {
     {
       at::AutoGradMode off(false);
       const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+      check_no_tangent(g[0], "confidence_xent backward");
       const Tensor dloss = g[0].to(torch::kFloat32).contiguous();
       LogProbGradArgs a{};
       a.x = x.data_ptr();
@@ -1376,6 +1384,7 @@ Tensor confidence_xent(Tensor x, Tensor labels, double weight, int64_t ignore) {
 
 // ------------------------------------------------------------------------------------------ dropout
 Tensor dropout_run(const Tensor& x0, const Tensor& key, int64_t cut) {
+  check_no_tangent(x0, "dropout");
   const Tensor x = x0.contiguous();
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
   Tensor y = torch::empty_like(x);

@@ -10,6 +10,7 @@ epilogue is fused).  Layers that read the same activations share ``quantize_rows
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .common import on_gpu, ext
 
@@ -99,6 +100,12 @@ class Int8Rows:
         return (q.float() * self.scale[:, None]).view(self.shape)
 
 
+def _no_tangent(who, *tensors):
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{who}: inference only, no forward-mode derivative")
+
+
 def _check_rows(x, who):
     if x.dim() < 1:
         raise ValueError(f"{who}: x [..., K], got a scalar")
@@ -106,6 +113,7 @@ def _check_rows(x, who):
         raise TypeError(f"{who}: bf16 / fp32 activations, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who}: inference only (torch.no_grad(), or a tensor without gradient)")
+    _no_tangent(who, x)
     _check_k(x.shape[-1])
 
 
@@ -140,6 +148,7 @@ def int8_linear(x, weight, bias=None, residual=None, relu=False):
     device = (x if rows is None else rows.scale).device
     if device != weight.device:
         raise ValueError(f"int8_linear: x on {device}, weight on {weight.device}")
+    _no_tangent("int8_linear", bias, residual)
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (weight.n,) or bias.device != device:
             raise ValueError(f"int8_linear: bias fp32 [{weight.n}] on {device}, got {bias.dtype} "

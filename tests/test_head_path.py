@@ -627,3 +627,41 @@ def test_gpu_dropout_start_at_reaches_a_captured_step(gpu):
             graph.replay()
             keep = ref_dropout_keep(5000, 0.5, torch.tensor([5, first + i]))
             assert torch.equal(out.cpu() != 0, keep)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_forward_mode_derivatives_are_not_dropped(device):
+    """A tangent comes out (the log-probabilities and the loss on the CPU) or the call is refused."""
+    import torch.autograd.forward_ad as fw
+    x, v = torch.randn(4, 50, device=device), torch.randn(4, 50, device=device)
+    y, key = torch.arange(4, device=device), torch.zeros(2, dtype=torch.int64, device=device)
+    w = ops.Int8Weight.quantize(torch.randn(50, 50, device=device))
+    b = torch.ones(50, device=device)
+    with fw.dual_level():
+        d, db = fw.make_dual(x, v), fw.make_dual(b, b)
+        calls = {"log_probs": lambda: ops.label_log_probs(d, y).log_prob,
+                 "loss": lambda: ops.confidence_penalty_cross_entropy(d, y, 0.1),
+                 "dropout": lambda: ops.dropout(d, 0.5, key), "rows": lambda: ops.quantize_rows(d),
+                 "x": lambda: ops.int8_linear(d, w), "bias": lambda: ops.int8_linear(x, w, db),
+                 "residual": lambda: ops.int8_linear(x, w, None, d)}
+        for name, f in calls.items():
+            if device == "cpu" and name in ("log_probs", "loss"):
+                t = fw.unpack_dual(f()).tangent
+                xg = x.clone().requires_grad_(True)
+                o = (ops.label_log_probs(xg, y).log_prob if name == "log_probs" else
+                     ops.confidence_penalty_cross_entropy(xg, y, 0.1))
+                want = (torch.autograd.grad(o.sum(), xg)[0] * v).sum()
+                assert abs(float(t.sum()) - float(want)) < 1e-4
+            else:
+                with pytest.raises(RuntimeError):
+                    f()
+        # a backward pass over tangents (forward over reverse)
+        if device != "cpu":
+            xg = x.clone().requires_grad_(True)
+            for o in (ops.label_log_probs(xg, y).log_prob, ops.label_log_probs(xg, None, 2).top_log_prob,
+                      ops.dropout(xg, 0.5, key), ops.confidence_penalty_cross_entropy(xg, y, 0.1)):
+                one = torch.ones_like(o)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(o, xg, fw.make_dual(one, one))
+        assert torch.equal(ops.int8_linear(x, w, b), ops.int8_linear(fw.unpack_dual(d).primal, w, b))
+    ops.dropout(x, 0.5, key)
