@@ -375,8 +375,8 @@ __device__ __forceinline__ RowGrad row_grad(const LogProbGradArgs& a, long row) 
     g = a.g_logp ? a.g_logp[row] : 0.f;
     r.h = a.g_ent ? a.g_ent[row] : 0.f;
   }
-  // a label out of range had log p = NaN: so has its gradient
-  r.g = !lab || !counts ? 0.f : r.y < 0 || r.y >= a.C ? NAN : g;
+  // a label out of range had log p = NaN: so is a gradient through it
+  r.g = !lab || !counts ? 0.f : g != 0.f && (r.y < 0 || r.y >= a.C) ? NAN : g;
   if (!counts) r.y = -1;
   const bool empty = r.logs == INFINITY;
   if (empty) r.g = r.h = 0.f;  // nothing depends on the logits

@@ -48,9 +48,11 @@ def ref_label_log_probs(logits, labels=None, top_k=0, ignore_index=-100, dtype=t
     lp = torch.where(bad[..., None], nan[..., None], lp)
     logp = tlp = ti = None
     if labels is not None:
-        ok = (labels >= 0) & (labels < C)
+        ok = ((labels >= 0) & (labels < C)) | (labels == ignore_index)
         got = lp.gather(-1, labels.clamp(0, C - 1).unsqueeze(-1)).squeeze(-1)
-        got = torch.where(ok, got, nan)
+        got = got + torch.where(ok, torch.zeros_like(got), nan)
+        if got.requires_grad:  # a gradient through a label out of range is NaN (a selection would pass 0)
+            got.register_hook(lambda g: None if g is None else torch.where(ok | (g == 0), g, nan))
         logp = torch.where(labels == ignore_index, torch.zeros_like(got), got)
     if top_k:
         keys = torch.where(bad[..., None], torch.zeros_like(x), x)
@@ -107,8 +109,9 @@ def label_log_probs(logits, labels=None, top_k=0, ignore_index=-100):
 
     A class is masked with −inf.  A row with every class masked gives log-probabilities of −inf,
     entropy 0 and no gradient.  A label equal to ``ignore_index`` (checked first) gives
-    log-probability 0 and no gradient through it; any other label outside [0, C) gives NaN.  A row
-    with a NaN or +inf gives NaN throughout and the indices 0 … top_k − 1.
+    log-probability 0 and no gradient through it; any other label outside [0, C) gives NaN, and the
+    row's gradient is NaN where one that is not zero arrives at that log-probability.  A row with a
+    NaN or +inf gives NaN throughout and the indices 0 … top_k − 1.
     """
     x, lab, lead = flat_rows(logits, labels, top_k, "label_log_probs")
     if not on_gpu(logits):

@@ -356,3 +356,31 @@ def test_gpu_longest_row(gpu):
     assert float(d[0, C - 1]) == 1.0
     lo, hi = float(d[0, :C - 1].min()), float(d[0, :C - 1].max())
     assert lo == hi and abs(lo * C + 1) <= 2.0 ** -8 + 2.0 ** -17  # bf16; exp of a log to 2^-22 x 22
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("C", [5, 300, 2500])
+def test_gradient_of_labels_out_of_range(C, device):
+    """NaN in the whole row where a gradient arrives at such a label's log-probability, none where
+    it is zero or another output's; ignored and empty rows have none."""
+    x = torch.randn(6, C, generator=torch.Generator().manual_seed(C))
+    x[5] = -INF
+    y = torch.tensor([1, C, -7, -100, 2 ** 40, C + 3], device=device)
+    x = x.to(device).requires_grad_(True)
+    bad = torch.tensor([False, True, True, False, True, False])
+
+    def grad(f, *g):
+        return torch.autograd.grad(f(), x, *g)[0].cpu()
+    d = grad(lambda: ops.label_log_probs(x, y).log_prob.sum())
+    assert torch.equal(d.isnan().all(1), bad) and torch.equal(d.isnan().any(1), bad)
+    assert bool((d[[3, 5]] == 0).all()) and bool((d[0] != 0).any())
+    for k in (0, 2):
+        d = grad(lambda: ops.label_log_probs(x, y, top_k=k).log_prob,
+                 torch.tensor([1.0, 0, 0, 1, -2, 0], device=device))
+        assert d.isnan().all(1).tolist() == [False] * 4 + [True, False] and bool(d[:4].isfinite().all())
+        assert bool((d[1:4] == 0).all())
+    assert bool(grad(lambda: ops.label_log_probs(x, y, top_k=2).entropy.sum()).isfinite().all())
+    loss = ops.confidence_penalty_cross_entropy(x, y, 0.1)
+    assert bool(loss.isnan())
+    d = grad(lambda: loss)
+    assert torch.equal(d.isnan().all(1), bad) and torch.equal(d.isnan().any(1), bad)
