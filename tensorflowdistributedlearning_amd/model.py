@@ -57,6 +57,7 @@ from .engine import schedules
 from .models.deeplab import DeepLabResNet
 from . import models as _models
 from .models.params import FlatParams
+from .ops.dropout import check_layer_p
 from .ops.logprob import label_log_probs, MAX_TOP_K
 from .ops.loss import (confidence_penalty_cross_entropy, lovasz_hinge, softmax_cross_entropy,
                        softmax_eval)
@@ -173,11 +174,9 @@ class Model:
         self.fp8 = kwargs.get("fp8", False)
         # classifiers: dropout of the pooled features, weight of the entropy term of the loss
         # (ops/loss.confidence_penalty_cross_entropy), 8-bit linear layers in predictions
-        self.dropout = float(kwargs.get("dropout", 0.0))
+        self.dropout = check_layer_p(kwargs.get("dropout", 0.0))
         self.entropy_weight = float(kwargs.get("entropy_weight", 0.0))
         self.int8 = bool(kwargs.get("int8", False))
-        if not 0.0 <= self.dropout < 1.0:
-            raise ValueError(f"dropout: 0 <= p < 1, got {self.dropout}")
         if seg and (self.dropout or self.entropy_weight or self.int8):
             raise ValueError("dropout, entropy_weight and int8 are for the classifiers")
         # HIP-graph capture of each fold's training step ("auto": GPU runs whose collectives, if

@@ -22,7 +22,7 @@ from ..ops.dwconv import depthwise_conv2d
 from ..ops import bnconv
 from ..ops.bnconv import DeferredBNAct, bn_act_conv
 from ..ops.common import compute_weight, export_impl, flat_view
-from ..ops.dropout import dropout, DropoutKeys
+from ..ops.dropout import check_layer_p, dropout, DropoutKeys
 from ..ops.int8 import Int8Weight, int8_linear
 from ..ops.fp8 import DelayedScaler, flat_weights_for, transpose_weight
 from . import params as _params
@@ -743,9 +743,7 @@ class Dropout(nn.Module):
 
     def __init__(self, p, seed=None):
         super().__init__()
-        if not 0.0 <= p < 1.0:
-            raise ValueError(f"Dropout: 0 <= p < 1, got {p}")
-        self.p = float(p)
+        self.p = check_layer_p(p)
         self.seed = int(torch.randint(0, 2 ** 62, ()).item()) if seed is None else int(seed)
         self.first = 0
         self.__dict__["_streams"] = {}  # by device; kept: captured steps go on drawing from them

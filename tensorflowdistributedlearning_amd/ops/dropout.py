@@ -19,7 +19,18 @@ _M32 = 0xFFFFFFFF
 def _cut(p):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: 0 <= p <= 1, got {p}")
-    return round(65536 * float(p))
+    cut = round(65536 * float(p))
+    if cut == 65536 and p < 1:
+        raise ValueError(f"dropout: p is a multiple of 2^-16, and {p} rounds to 1, which keeps nothing")
+    return cut
+
+
+def check_layer_p(p):
+    """``p`` as a layer takes it: below 1, also as rounded."""
+    if p == 1:
+        raise ValueError("dropout: 0 <= p < 1, got 1")
+    _cut(p)
+    return float(p)
 
 
 def ref_philox4x32(c, k, rounds=10):
@@ -71,7 +82,8 @@ def dropout(x, p, key):
     """``x`` (bf16 / fp32, any shape) with each element zeroed with probability ``p`` (a multiple of
     2^-16, rounded) and the others scaled by 1 / (1 − p).  ``key``: int64 [2] on x's device, the seed
     and the call number; equal keys give equal masks.  Changing ``key`` in place between the forward
-    and the backward pass is an error (autograd's version check).  p = 0 returns ``x`` itself."""
+    and the backward pass is an error (autograd's version check).  A p that is or rounds to 0 returns
+    ``x`` itself; p = 1 drops everything, a p that only rounds to it is refused."""
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"dropout: bf16 / fp32 input, got {x.dtype}")
     if key.dtype != torch.int64 or key.shape != (2,):

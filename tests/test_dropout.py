@@ -173,3 +173,27 @@ def test_gpu_graph_draws_new_masks(gpu):
         masks.append(out[1].detach().clone())
     assert calls == list(range(1, 9))
     assert not any(torch.equal(masks[0], m) for m in masks[1:])
+
+
+def test_probabilities_that_round_to_one_are_refused():
+    """p < 1 within half a step (2^-17) of 1 would drop everything; p = 1 does so by name."""
+    from tensorflowdistributedlearning_amd.models.layers import Dropout
+    x, k = torch.ones(70000), key_of(1, 0)
+    for p in (0.999995, 1 - 2.0 ** -17, 1 - 2.0 ** -53):
+        with pytest.raises(ValueError):
+            ops.dropout(x, p, k)
+        with pytest.raises(ValueError):
+            Dropout(p)
+    p = 1 - 2.0 ** -16
+    y = ops.dropout(x, p, k)
+    keep = ref_dropout_keep(70000, p, k)
+    assert torch.equal(y, keep * 65536.0) and torch.equal(Dropout(p, seed=1)(x), y)
+    assert bool((ops.dropout(x, 1.0, k) == 0).all())
+    assert ops.dropout(x, 2.0 ** -18, k) is x  # rounds to 0: nothing is dropped
+
+
+def test_model_refuses_a_dropout_that_rounds_to_one(tmp_path):
+    from tensorflowdistributedlearning_amd.model import Model
+    with pytest.raises(ValueError):
+        Model(str(tmp_path / "m"), "none", n_gpus=1, n_fold=2, arch="resnet18", image_size=32, num_classes=4,
+              synthetic=True, device="cpu", save_best=0, export_format="none", dropout=0.999995)
