@@ -632,11 +632,16 @@ class ConvBN(nn.Module):
             else:
                 y, stats = bn_act_conv(x, self.conv, want_stats=True)
                 return self._bn_out(y, stats, residual, res_join, into, defer)
+        if not self.training and not torch.is_grad_enabled() and bn_fold_enabled():
+            if self.conv.int8_active() and (into is None or residual is None):
+                w8, bf = self.folded_int8(x.dtype, x.device)
+                y = int8_linear(x, w8, bias=bf, residual=residual, relu=self.relu)
+                if into is None:
+                    return y
+                into[0][..., into[1]:into[1] + y.shape[-1]].copy_(y)
+                return into[0]
         if (not self.training and into is None and not torch.is_grad_enabled()
                 and bn_fold_enabled()):
-            if self.conv.int8_active():
-                w8, bf = self.folded_int8(x.dtype, x.device)
-                return int8_linear(x, w8, bias=bf, residual=residual, relu=self.relu)
             wf, bf = self.folded_params(x.dtype, x.device)
             return self.conv.forward_folded(x, wf, bf, self.relu, residual)
         if self.training:

@@ -665,3 +665,26 @@ def test_forward_mode_derivatives_are_not_dropped(device):
                     torch.autograd.grad(o, xg, fw.make_dual(one, one))
         assert torch.equal(ops.int8_linear(x, w, b), ops.int8_linear(fw.unpack_dual(d).primal, w, b))
     ops.dropout(x, 0.5, key)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("arch", ["xception41", "deeplab", "resnet18"])
+def test_enable_int8_counts_the_layers_it_turns(arch, device, monkeypatch):
+    from tensorflowdistributedlearning_amd.models import layers
+    torch.manual_seed(12)
+    if arch == "deeplab":  # five of its ConvBNs write into a slice of a concatenation
+        m, x = models.DeepLabResNet(model_name="m", input_shape=(101, 101)), torch.randn(1, 101, 101, 2)
+    else:
+        m, x = models.build(arch, num_classes=6), torch.randn(1, 64, 64, 3)
+    m = m.to(device).eval()
+    if device == "cuda":
+        x = torch.nn.functional.pad(x, (0, 8 - x.shape[-1])).to(device, torch.bfloat16)
+    real, used = layers.int8_linear, set()
+    monkeypatch.setattr(layers, "int8_linear", lambda a, w, **k: (used.add(w), real(a, w, **k))[1])
+    with torch.no_grad():
+        full = m(x)
+        assert models.enable_int8(m, pointwise=True) > 0 and not used
+        y = m(x)
+        assert len(used) == models.enable_int8(m, pointwise=True)
+    cos = torch.nn.functional.cosine_similarity(y.float().flatten(), full.float().flatten(), dim=0)
+    assert not torch.equal(y, full) and float(cos) > 0.98
