@@ -547,9 +547,10 @@ void quantize_groups(const T* x, long ld, long M, long K, int8_t* q, float* scal
 }
 template <typename T>
 void quantize(const T* x, long ld, long M, long K, int8_t* q, float* scale, hipStream_t st) {
-  // 4 rows per workgroup where 16 would leave CUs idle (256 × 4096 bf16: 4.2 us against 8.2; 4096 ×
-  // 4096: 12.2 against 10.6, whose 64-byte pieces of the blocks cost more) or hold too much of a row
-  // per wave (8192 × 8192: 33.5 against 42.2; 1024 × 8192 fp32 10.1 against 36.9)
+  // 4 rows per workgroup where 16 would leave CUs idle (256 × 4096 bf16: 4.4 us against 8.3; 4096 ×
+  // 4096: 12.2 against 10.7, whose 64-byte pieces of the blocks cost more) or hold too much of a row
+  // per wave (8192 × 8192: 34.8 against 41.2 on one input, 42 against 47 on inputs that the last-level
+  // cache does not hold; 1024 × 8192 fp32 9.5 against 36.9)
   const long few = sizeof(T) == 2 ? 160 * 16 : 96 * 16;
   if (K > 4096 || (K > 512 && M < few)) quantize_groups<T, 4>(x, ld, M, K, q, scale, st);
   else quantize_groups<T, 16>(x, ld, M, K, q, scale, st);
@@ -715,12 +716,13 @@ void gemm(const Int8GemmArgs& a, hipStream_t st) {
     return;
   }
   auto tiles = [&](long bm, long bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
-  // 256 × 256 reads LDS and L2 least (8192³ 515 us, 128 × 128 582; 16384 × 4096 → 1024 56 and 66) but
+  // 256 × 256 reads LDS and L2 least (8192³, 200 calls in a row: 407 us on uniform random bytes, 384 on
+  // rectified activations, 128 × 128 510 and 458; 16384 × 4096 → 1024 56 and 66) but
   // leaves one workgroup per CU, which short sums do not hide (50176 × 256 → 1024: 73 us against 55).
   // 64 × 64, 128 k per step, while 128 × 128 gives no more than a tile to every other CU (512 × 4096 →
   // 4096, 128 tiles: 15.3 us against 17.7; 1024 × 4096 → 4096, 256 tiles: 28 against 21).  The
   // 32×32×32 form of the matrix unit wins on the smaller tiles (2049 × 1999 → 1003 on 128 × 128: 14.3
-  // us against 19.5), the 16×16×64 form on the large one (8192³: 522 against 527 us).
+  // us against 19.5), the 16×16×64 form on the large one (8192³: 407 against 433 us, 384 against 389).
   if (tiles(256, 256) >= 180 && a.Kp >= 1024) run_gemm<T, 16, 8, 4, 2, 4, 1, 4>(a, st);
   else if (tiles(128, 128) > 128) run_gemm<T, 32, 4, 2, 2, 4, 1, 4>(a, st);
   else run_gemm<T, 32, 2, 2, 2, 2, 2, 4>(a, st);

@@ -118,9 +118,10 @@ def enable_int8(model, pointwise=False):
     """8-bit inference (ops/int8.py) of the linear layers: in eval mode without autograd their
     weights are quantised once per parameter version, their input rows on the fly.  Few rows (serving
     one image) are a stream over the weights, half as long in 8 bits.  ``pointwise``: also every
-    1×1, stride-1, unpadded ConvBN, BN folded (a pass over the activations quantises them, which a
-    bf16 product does not need: half the weights' memory, not less time, at these networks'
-    sizes).  Training, evaluation with autograd and servable exports are unaffected.  Returns the
+    1×1, stride-1, unpadded ConvBN, BN folded.  A pass over the activations quantises them, which a
+    bf16 product does not need: ResNet-50 as a graph gains at batch 1 (1,254 images/s, linear layer
+    alone 1,291, with the 1×1 convs 1,438) and loses at 32 (28,199, 28,959, 27,780) and 256 (54,304,
+    54,493, 50,573).  Training, evaluation with autograd and servable exports are unaffected.  Returns the
     number of layers."""
     from .layers import ConvBN, Linear, RowPackedConv2d, resolve_padding
     n = 0
